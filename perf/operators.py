@@ -183,7 +183,7 @@ def prepare(case, seed):
         else:
             state["rows"] = normal(L, d, dtype=dtype)
             state["gates"] = gates
-            state["places"], state["loads"] = _order(picks, case["paths"])
+            state["places"], _ = _order(picks, case["paths"])
             if case["train"]:
                 state["rows"].requires_grad_()
                 state["gates"].requires_grad_()
@@ -226,14 +226,15 @@ def prepare(case, seed):
 
 # --------------------------------------------------------------------------- the plain forms
 def _order(picks, paths):
-    """places [T, k] and loads [E] of a stable sort by path; -1 for picks that are no path."""
+    """places [T, k] and loads [E] of a stable sort by path.  Picks that are no path come last;
+    -2 - row stands for them: the row that stays empty in their place."""
     flat = picks.reshape(-1).long()
     valid = (flat >= 0) & (flat < paths)
     key = torch.where(valid, flat, paths)
     order = torch.argsort(key, stable=True)
     places = torch.empty_like(flat)
     places[order] = torch.arange(flat.numel(), device=flat.device)
-    places = torch.where(valid, places, -1)
+    places = torch.where(valid, places, -2 - places)
     loads = torch.zeros(paths + 1, dtype=torch.int32, device=flat.device)
     loads.index_add_(0, key, torch.ones_like(key, dtype=torch.int32))
     return places.view(picks.shape).to(torch.int32), loads[:paths]
@@ -352,15 +353,15 @@ def _framework(state):
     if op == "sort":
         places, loads = router.order_picks(state["picks"], case["paths"])
         if case["fp8"]:
-            rows, scales = router.sort_cells_fp8(state["cells"], places, loads)
+            rows, scales = router.sort_cells_fp8(state["cells"], places)
             return places, loads, rows, scales
-        rows = router.sort_cells(state["cells"], places, loads)
+        rows = router.sort_cells(state["cells"], places)
         if not case["train"]:
             return places, loads, rows
         (grad,) = torch.autograd.grad(rows, state["cells"], state["row_grads"])
         return places, loads, rows.detach(), grad
     if op == "unsort":
-        out = router.unsort_cells(state["rows"], state["places"], state["loads"], state["gates"])
+        out = router.unsort_cells(state["rows"], state["places"], state["gates"])
         if not case["train"]:
             return out
         grads = torch.autograd.grad(out, (state["rows"], state["gates"]), state["cell_grads"])
