@@ -717,3 +717,197 @@ def combine_with_indices_and_loads(
                 tags_value = tags_value.narrow(0, 1, n - 1)
         out_loads = torch.tensor([tags_value.numel()], dtype=torch.int32, device=dev)
         return [out, tags_value, out_loads]
+
+
+# ---------------------------------------------------------------- routing by compact picks
+#
+# The picks of a top-k, [cells, k], instead of a [cells, paths] mask: rows sorted by path without a
+# host read (there are cells * k of them whatever the loads are), and their gradients.
+
+
+def order_picks(picks: torch.Tensor, path_num: int):
+    """Where each pick of a top-k goes in a buffer of rows sorted by path.
+
+    ``picks`` [cells, k], int32 or int64 (the indices that ``torch.topk`` returns); the same path
+    twice is two rows.  Returns (places [cells, k] int32, loads [path_num] int32): path e has the
+    rows from ``loads[:e].sum()`` on, in the order of the cells.  Picks outside ``[0, path_num)``
+    go nowhere; their places are ``-2 - row``, naming the row at the end of the buffer that stays
+    empty.  A place may be set to -1 afterwards to leave out a pick altogether.  At most 1024
+    paths; nothing is read back to the host."""
+    _check_cuda(picks, "picks")
+    if picks.dim() != 2 or picks.size(1) < 1:
+        raise RuntimeError(f"picks must be [cells, k], got {tuple(picks.shape)}")
+    if picks.dtype not in (torch.int32, torch.int64):
+        raise RuntimeError(f"picks must be int32 or int64, got {picks.dtype}")
+    path_num = int(path_num)
+    dev = picks.device
+    with _lib.device_guard(dev):
+        picks = picks if picks.is_contiguous() else picks.contiguous()
+        total = picks.numel()
+        places = torch.empty(picks.shape, dtype=torch.int32, device=dev)
+        loads = torch.empty((max(path_num, 0),), dtype=torch.int32, device=dev)
+        nbytes = _lib.query("brt_pick_order_scratch_bytes", total, path_num)
+        # of its own for each call: a graph that holds the call may run beside another one's
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        _lib.call("brt_order_picks", _ptr(picks), int(picks.dtype == torch.int64), total, path_num,
+                  _ptr(places), _ptr(loads), _ptr(scratch), nbytes, _stream(dev))
+    return places, loads
+
+
+def _check_places(places: torch.Tensor, like: torch.Tensor, name: str) -> torch.Tensor:
+    _check_cuda(like, name)
+    _check_cuda(places, "places")
+    if places.dtype != torch.int32 or places.dim() != 2 or places.size(1) < 1:
+        raise RuntimeError("places must be the [cells, k] int32 tensor of order_picks")
+    if places.device != like.device:
+        raise RuntimeError(f"{name} and places are on different devices")
+    if like.dtype not in _DT:
+        raise NotImplementedError("data type is not supported")
+    if like.dim() < 1:
+        raise RuntimeError(f"{name} has no first dimension")
+    return places if places.is_contiguous() else places.contiguous()
+
+
+def _cell_size(shape) -> int:
+    size = 1
+    for n in shape[1:]:
+        size *= n
+    return size
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """``t`` contiguous and on a 16-byte boundary."""
+    if not t.is_contiguous():
+        return t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _sort(in_data, places):
+    T, k = places.shape
+    size = _cell_size(in_data.shape)
+    with _lib.device_guard(in_data.device):
+        src = in_data if in_data.is_contiguous() else in_data.contiguous()
+        rows = torch.empty((T * k,) + tuple(in_data.shape[1:]), dtype=in_data.dtype,
+                           device=in_data.device)
+        if rows.numel():
+            _lib.call("brt_sort_cells", _ptr(src), _ptr(places), _ptr(rows), T, k, size,
+                      _DT[in_data.dtype], _stream(in_data.device))
+    return rows
+
+
+def _unsort(rows, places, gates):
+    T, k = places.shape
+    size = _cell_size(rows.shape)
+    with _lib.device_guard(rows.device):
+        src = rows if rows.is_contiguous() else rows.contiguous()
+        g = gates if gates is None or gates.is_contiguous() else gates.contiguous()
+        out = torch.empty((T,) + tuple(rows.shape[1:]), dtype=rows.dtype, device=rows.device)
+        if out.numel():
+            _lib.call("brt_unsort_cells", _ptr(src), _ptr(places), _ptr(g), _ptr(out), T, k, size,
+                      _DT[rows.dtype], 0 if g is None else _DT[g.dtype], _stream(rows.device))
+    return out
+
+
+class _SortCells(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, in_data, places):
+        ctx.save_for_backward(places)
+        return _sort(in_data, places)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, row_grads):
+        (places,) = ctx.saved_tensors
+        return _unsort(row_grads, places, None), None
+
+
+class _UnsortCells(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, rows, places, gates):
+        # the rows are only read again for the gradient of the gates
+        keep = rows if ctx.needs_input_grad[2] else None
+        ctx.save_for_backward(keep, places, gates)
+        return _unsort(rows, places, gates)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, cell_grads):
+        rows, places, gates = ctx.saved_tensors
+        if gates is None:
+            return _sort(cell_grads, places), None, None
+        T, k = places.shape
+        dev = cell_grads.device
+        with _lib.device_guard(dev):
+            grads = cell_grads if cell_grads.is_contiguous() else cell_grads.contiguous()
+            g = gates if gates.is_contiguous() else gates.contiguous()
+            row_grads = gate_grads = None
+            if ctx.needs_input_grad[0]:
+                row_grads = torch.empty((T * k,) + tuple(grads.shape[1:]), dtype=grads.dtype,
+                                        device=dev)
+            if ctx.needs_input_grad[2]:
+                rows = rows if rows.is_contiguous() else rows.contiguous()
+                gate_grads = torch.empty((T, k), dtype=g.dtype, device=dev)
+            if grads.numel():
+                _lib.call("brt_unsort_cells_backward", _ptr(grads), _ptr(rows), _ptr(places),
+                          _ptr(g), _ptr(row_grads), _ptr(gate_grads), T, k,
+                          _cell_size(grads.shape), _DT[grads.dtype], _DT[g.dtype], _stream(dev))
+            elif gate_grads is not None:
+                gate_grads.zero_()
+        return row_grads, None, gate_grads
+
+
+def sort_cells(in_data: torch.Tensor, places: torch.Tensor) -> torch.Tensor:
+    """``rows[places[t, j]] = in_data[t]``: cells [cells, ...] to [cells * k, ...] rows sorted by
+    path, ``places`` as ``order_picks`` returned them.  Rows that stay empty are zeros.  The
+    gradient of a cell is the sum of its rows' gradients (fp32, rounded once)."""
+    places = _check_places(places, in_data, "in_data")
+    if in_data.size(0) != places.size(0):
+        raise RuntimeError(f"{in_data.size(0)} cells but places of {places.size(0)}")
+    if in_data.requires_grad and torch.is_grad_enabled():
+        return _SortCells.apply(in_data, places)
+    return _sort(in_data, places)
+
+
+def sort_cells_fp8(in_data: torch.Tensor, places: torch.Tensor):
+    """``sort_cells`` followed by ``quantize_rows`` of ``_C.expert`` in one pass over the cells:
+    (codes [cells * k, width] float8_e4m3fn, scales [cells * k, ceil(width / 128)] fp32).  The
+    width must be a multiple of 16.  No gradient: train through ``sort_cells``."""
+    places = _check_places(places, in_data, "in_data")
+    if in_data.dim() != 2 or in_data.size(0) != places.size(0):
+        raise RuntimeError(f"in_data must be [{places.size(0)}, width], got "
+                           f"{tuple(in_data.shape)}")
+    if in_data.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("sort_cells_fp8 has no gradient: use sort_cells, or no_grad()")
+    T, k = places.shape
+    width = in_data.size(1)
+    if width < 1 or width % 16 != 0:
+        raise NotImplementedError(f"the width must be a multiple of 16, got {width}")
+    dev = in_data.device
+    with _lib.device_guard(dev):
+        src = _aligned(in_data)
+        codes = torch.empty((T * k, width), dtype=torch.float8_e4m3fn, device=dev)
+        scales = torch.empty(((width + 127) // 128, T * k), dtype=torch.float32, device=dev)
+        _lib.call("brt_sort_cells_fp8", _ptr(src), _ptr(places), _ptr(codes), _ptr(scales), T, k,
+                  width, _DT[in_data.dtype], _stream(dev))
+    return codes, scales.t()
+
+
+def unsort_cells(rows: torch.Tensor, places: torch.Tensor,
+                 gates: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``out[t] = sum over j of gates[t, j] * rows[places[t, j]]``: rows back to their cells, zeros
+    for a cell whose picks all go nowhere.  ``gates`` [cells, k] fp32 or of the rows' type (their
+    values at picks that go nowhere do not matter), or None for the plain sum.  fp32 sums in the
+    order of j, rounded once.  Differentiable in rows and gates; empty rows get zero gradients."""
+    places = _check_places(places, rows, "rows")
+    if rows.size(0) != places.numel():
+        raise RuntimeError(f"{rows.size(0)} rows but {places.numel()} places")
+    if gates is not None:
+        _check_cuda(gates, "gates")
+        if gates.shape != places.shape or gates.device != rows.device:
+            raise RuntimeError("gates must have the shape and device of places")
+        if gates.dtype not in (torch.float32, rows.dtype):
+            raise RuntimeError("gates must be float32 or match the data type")
+    if torch.is_grad_enabled() and (rows.requires_grad or
+                                    (gates is not None and gates.requires_grad)):
+        return _UnsortCells.apply(rows, places, gates)
+    return _unsort(rows, places, gates)

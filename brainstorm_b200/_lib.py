@@ -61,6 +61,20 @@ SIGNATURES = {
     "brt_sum_rows_by_index": (_int, [_vp, _vp, _vp, _i64, _i64, _i64, _int, _vp, _sz, _vp]),
     "brt_grouped_expert_gemm": (_int, [_vp, _vp, _vp, _vp, _int, _i64, _i32, _i64, _i64, _int,
                                        _vp, _vp]),
+    "brt_pick_order_scratch_bytes": (_sz, [_i64, _int]),
+    "brt_order_picks": (_int, [_vp, _int, _i64, _int, _vp, _vp, _vp, _sz, _vp]),
+    "brt_sort_cells": (_int, [_vp, _vp, _vp, _i64, _int, _i64, _int, _vp]),
+    "brt_sort_cells_fp8": (_int, [_vp, _vp, _vp, _vp, _i64, _int, _i64, _int, _vp]),
+    "brt_unsort_cells": (_int, [_vp, _vp, _vp, _vp, _i64, _int, _i64, _int, _int, _vp]),
+    "brt_unsort_cells_backward": (
+        _int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _int, _i64, _int, _int, _vp]),
+    "brt_quantize_rows": (_int, [_vp, _vp, _vp, _i64, _i64, _int, _vp]),
+    "brt_quantize_expert_weights": (_int, [_vp, _vp, _vp, _int, _i64, _i64, _int, _int, _vp]),
+    "brt_grouped_expert_gemm_fp8": (
+        _int, [_vp, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _int, _i64, _i32, _i64, _i64, _int, _int,
+               _vp, _vp]),
+    "brt_grouped_expert_weight_grad": (
+        _int, [_vp, _vp, _vp, _vp, _int, _i64, _i32, _i64, _i64, _int, _vp, _vp]),
     "brt_locality_reorder": (_int, [_vp, _int, _vp, _vp, _vp]),
     "brt_group_locality_reorder": (_int, [_vp, _int, _int, _vp, _vp, _vp]),
     "brt_nccl_get_unique_id": (_int, [_vp]),

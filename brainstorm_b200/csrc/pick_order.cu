@@ -1,0 +1,284 @@
+// Order of the rows of a mixture-of-experts layer from compact picks (the indices of a top-k).
+//
+//   loads[e]     = number of picks that are e
+//   places[t, j] = loads[0] + .. + loads[e-1] + number of earlier picks that are e
+//                  (earlier: a smaller t * k + j), for e = picks[t, j]
+//
+// A stable counting sort.  Picks outside [0, paths) go nowhere: they count as one more path
+// behind the last, and -2 - row stands in their place, the row at the end that stays empty for
+// them.  Integer sums in a fixed order: the result does not depend on timing.
+//
+// A CTA owns a tile of consecutive picks and each of its warps a run of them.  Counting: a
+// histogram per warp in shared memory; the lanes of a step that share a path are found with one
+// match instruction and their first lane adds for all.  The exclusive sums over paths, tiles and
+// warps turn the histograms into next places, and a second walk over the picks hands them out.
+// Up to kOneCta picks one CTA does all of it in one launch; more take two launches, tile
+// counts in between (the second launch is set up under the first).
+#include "common.cuh"
+
+namespace brt_b200 {
+namespace {
+
+constexpr int kMaxPaths = 1024;
+constexpr int kWarps = 32;
+constexpr int kOneCta = 8192;
+constexpr int kTileMin = 2048;
+
+struct OrderArgs {
+  const void* picks;
+  int* places;
+  int* loads;
+  int* counts;  // [tiles, paths + 1], two-launch form
+  int n;
+  int paths;
+  int tile;  // picks per CTA, a multiple of 32 * warps
+  int tiles;
+};
+
+template <typename P>
+__device__ __forceinline__ int bucket_of(const P* picks, int i, int paths) {
+  const P v = picks[i];
+  return v >= 0 && v < (P)paths ? (int)v : paths;
+}
+
+// s_hist[warp][bucket] of this CTA's tile.
+template <typename P>
+__device__ __forceinline__ void count_tile(const OrderArgs& a, int* s_hist, int lo, int hi) {
+  const int buckets = a.paths + 1;
+  const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int i = threadIdx.x; i < warps * buckets; i += blockDim.x) s_hist[i] = 0;
+  __syncthreads();
+  const P* picks = static_cast<const P*>(a.picks);
+  const int run = a.tile / warps;
+  const int end = min(lo + (warp + 1) * run, hi);
+  int* const mine = s_hist + warp * buckets;
+  for (int i0 = lo + warp * run; i0 < end; i0 += 32) {
+    const int i = i0 + lane;
+    const int b = i < end ? bucket_of(picks, i, a.paths) : buckets;
+    const unsigned same = __match_any_sync(0xffffffffu, b);
+    if (b < buckets && lane == __ffs(same) - 1) mine[b] += __popc(same);
+    __syncwarp();
+  }
+  __syncthreads();
+}
+
+// s_hist[warp][bucket] holds the next place of every warp and bucket: hands them out.
+template <typename P>
+__device__ __forceinline__ void place_tile(const OrderArgs& a, int* s_hist, int lo, int hi) {
+  const int buckets = a.paths + 1;
+  const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const P* picks = static_cast<const P*>(a.picks);
+  const int run = a.tile / warps;
+  const int end = min(lo + (warp + 1) * run, hi);
+  int* const mine = s_hist + warp * buckets;
+  for (int i0 = lo + warp * run; i0 < end; i0 += 32) {
+    const int i = i0 + lane;
+    const int b = i < end ? bucket_of(picks, i, a.paths) : buckets;
+    const unsigned same = __match_any_sync(0xffffffffu, b);
+    int row = 0;
+    if (b < buckets) row = mine[b] + __popc(same & ((1u << lane) - 1));
+    __syncwarp();
+    if (b < buckets && lane == __ffs(same) - 1) mine[b] += __popc(same);
+    __syncwarp();
+    if (b < buckets) a.places[i] = b < a.paths ? row : -2 - row;
+  }
+}
+
+// s_base[bucket] <- exclusive sums of s_total over the buckets (one warp).
+__device__ __forceinline__ void scan_buckets(const int* s_total, int* s_base, int buckets) {
+  const int lane = threadIdx.x & 31;
+  int before = 0;
+  for (int b0 = 0; b0 < buckets; b0 += 32) {
+    const int b = b0 + lane;
+    const int mine = b < buckets ? s_total[b] : 0;
+    int incl = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, incl, d);
+      if (lane >= d) incl += up;
+    }
+    if (b < buckets) s_base[b] = before + incl - mine;
+    before += __shfl_sync(0xffffffffu, incl, 31);
+  }
+}
+
+template <typename P>
+__global__ void __launch_bounds__(kWarps * 32) pick_order_kernel(const OrderArgs a) {
+  extern __shared__ int s_mem[];
+  const int buckets = a.paths + 1, warps = blockDim.x >> 5;
+  int* const s_hist = s_mem;
+  int* const s_total = s_hist + warps * buckets;
+  int* const s_base = s_total + buckets;
+  count_tile<P>(a, s_hist, 0, a.n);
+  for (int b = threadIdx.x; b < buckets; b += blockDim.x) {
+    int sum = 0;
+    for (int w = 0; w < warps; w++) {
+      const int c = s_hist[w * buckets + b];
+      s_hist[w * buckets + b] = sum;
+      sum += c;
+    }
+    s_total[b] = sum;
+    if (b < a.paths) a.loads[b] = sum;
+  }
+  __syncthreads();
+  if (threadIdx.x < 32) scan_buckets(s_total, s_base, buckets);
+  __syncthreads();
+  for (int i = threadIdx.x; i < warps * buckets; i += blockDim.x) s_hist[i] += s_base[i % buckets];
+  __syncthreads();
+  place_tile<P>(a, s_hist, 0, a.n);
+}
+
+template <typename P>
+__global__ void __launch_bounds__(kWarps * 32) pick_count_kernel(const OrderArgs a) {
+  extern __shared__ int s_mem[];
+  const int buckets = a.paths + 1, warps = blockDim.x >> 5;
+  const int lo = blockIdx.x * a.tile, hi = min(lo + a.tile, a.n);
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  count_tile<P>(a, s_mem, lo, hi);
+  for (int b = threadIdx.x; b < buckets; b += blockDim.x) {
+    int sum = 0;
+    for (int w = 0; w < warps; w++) sum += s_mem[w * buckets + b];
+    a.counts[blockIdx.x * buckets + b] = sum;
+  }
+}
+
+template <typename P>
+__global__ void __launch_bounds__(kWarps * 32) pick_place_kernel(const OrderArgs a) {
+  extern __shared__ int s_mem[];
+  const int buckets = a.paths + 1, warps = blockDim.x >> 5;
+  int* const s_hist = s_mem;
+  int* const s_total = s_hist + warps * buckets;
+  int* const s_base = s_total + buckets;
+  int* const s_before = s_base + buckets;  // picks of the bucket in earlier tiles
+  const int lo = blockIdx.x * a.tile, hi = min(lo + a.tile, a.n);
+  for (int b = threadIdx.x; b < buckets; b += blockDim.x) s_total[b] = s_before[b] = 0;
+  count_tile<P>(a, s_hist, lo, hi);
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the tile counts are complete
+  // neighbouring threads take neighbouring buckets; the tiles are dealt out to groups of threads
+  const int groups = max(1, (int)blockDim.x / buckets);
+  for (int at = threadIdx.x; at < groups * buckets; at += blockDim.x) {
+    const int b = at % buckets;
+    int total = 0, before = 0;
+#pragma unroll 4
+    for (int t = at / buckets; t < a.tiles; t += groups) {
+      const int c = a.counts[t * buckets + b];
+      total += c;
+      if (t < (int)blockIdx.x) before += c;
+    }
+    atomicAdd(&s_total[b], total);  // integer sums: any order gives the same
+    atomicAdd(&s_before[b], before);
+  }
+  __syncthreads();
+  if (threadIdx.x < 32) scan_buckets(s_total, s_base, buckets);
+  __syncthreads();
+  for (int b = threadIdx.x; b < buckets; b += blockDim.x) {
+    int next = s_base[b] + s_before[b];
+    for (int w = 0; w < warps; w++) {
+      const int c = s_hist[w * buckets + b];
+      s_hist[w * buckets + b] = next;
+      next += c;
+    }
+    if (blockIdx.x == 0 && b < a.paths) a.loads[b] = s_total[b];
+  }
+  __syncthreads();
+  place_tile<P>(a, s_hist, lo, hi);
+}
+
+int tile_for(int64_t n) {
+  const int64_t tiles = sm_count();
+  int64_t tile = (n + tiles - 1) / tiles;
+  if (tile < kTileMin) tile = kTileMin;
+  return (int)round_up((size_t)tile, kWarps * 32);
+}
+
+template <typename P>
+int launch_order(OrderArgs a, cudaStream_t st) {
+  const int buckets = a.paths + 1;
+  static thread_local int configured_device = -1;
+  int dev = 0;
+  BRT_CUDA_TRY(cudaGetDevice(&dev));
+  if (configured_device != dev) {
+    const int most = (kWarps + 3) * (kMaxPaths + 1) * (int)sizeof(int);
+    BRT_CUDA_TRY(cudaFuncSetAttribute(pick_order_kernel<P>,
+                                      cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+    BRT_CUDA_TRY(cudaFuncSetAttribute(pick_count_kernel<P>,
+                                      cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+    BRT_CUDA_TRY(cudaFuncSetAttribute(pick_place_kernel<P>,
+                                      cudaFuncAttributeMaxDynamicSharedMemorySize, most));
+    configured_device = dev;
+  }
+  const KernelTimer timer("pick_order", st);
+  if (a.n <= kOneCta) {
+    int warps = (a.n + 31) / 32;
+    if (warps > kWarps) warps = kWarps;
+    a.tile = (int)round_up((size_t)a.n, (size_t)warps * 32);
+    const size_t smem = (size_t)(warps + 2) * buckets * sizeof(int);
+    pick_order_kernel<P><<<1, warps * 32, smem, st>>>(a);
+    note_launch();
+    BRT_LAUNCH_CHECK("pick_order_kernel");
+    return BRT_OK;
+  }
+  pick_count_kernel<P><<<a.tiles, kWarps * 32, (size_t)kWarps * buckets * sizeof(int), st>>>(a);
+  note_launch();
+  BRT_LAUNCH_CHECK("pick_count_kernel");
+  cudaLaunchAttribute early;
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3((unsigned)a.tiles);
+  config.blockDim = dim3(kWarps * 32);
+  config.dynamicSmemBytes = (size_t)(kWarps + 3) * buckets * sizeof(int);
+  config.stream = st;
+  config.attrs = &early;
+  config.numAttrs = 1;
+  BRT_CUDA_TRY(cudaLaunchKernelEx(&config, pick_place_kernel<P>, a));
+  note_launch();
+  BRT_LAUNCH_CHECK("pick_place_kernel");
+  return BRT_OK;
+}
+
+}  // namespace
+}  // namespace brt_b200
+
+using namespace brt_b200;
+
+extern "C" {
+
+BRT_API size_t brt_pick_order_scratch_bytes(int64_t pick_total, int path_num) {
+  if (pick_total <= kOneCta || path_num <= 0) return 0;
+  const int64_t tile = tile_for(pick_total);
+  return (size_t)((pick_total + tile - 1) / tile) * (size_t)(path_num + 1) * sizeof(int);
+}
+
+BRT_API int brt_order_picks(const void* picks, int picks_are_64bit, int64_t pick_total,
+                            int path_num, int32_t* places, int32_t* loads, void* scratch,
+                            size_t scratch_bytes, void* stream) {
+  clear_error();
+  BRT_REQUIRE(path_num > 0 && path_num <= kMaxPaths, "path_num %d outside [1, %d]", path_num,
+              kMaxPaths);
+  BRT_REQUIRE(pick_total >= 0 && pick_total < (1LL << 31) - (1 << 20),
+              "%lld picks: the rows are counted in 32 bits", (long long)pick_total);
+  BRT_REQUIRE(loads != nullptr, "loads is null");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (pick_total == 0) {
+    BRT_CUDA_TRY(cudaMemsetAsync(loads, 0, (size_t)path_num * sizeof(int), st));
+    return BRT_OK;
+  }
+  BRT_REQUIRE(picks != nullptr && places != nullptr, "null pointer argument");
+  const size_t need = brt_pick_order_scratch_bytes(pick_total, path_num);
+  if (need > 0 && (scratch == nullptr || scratch_bytes < need))
+    return set_error(BRT_ERR_SCRATCH_TOO_SMALL, "scratch holds %zu bytes, %zu are needed",
+                     scratch == nullptr ? (size_t)0 : scratch_bytes, need);
+  OrderArgs a;
+  a.picks = picks;
+  a.places = places;
+  a.loads = loads;
+  a.counts = static_cast<int*>(scratch);
+  a.n = (int)pick_total;
+  a.paths = path_num;
+  a.tile = tile_for(pick_total);
+  a.tiles = (a.n + a.tile - 1) / a.tile;
+  return picks_are_64bit ? launch_order<long long>(a, st) : launch_order<int>(a, st);
+}
+
+}  // extern "C"

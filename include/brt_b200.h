@@ -366,6 +366,105 @@ BRT_API int brt_grouped_expert_gemm(const void* rows, const void* weights, void*
                                     int64_t out_features, int relu, void* error_word,
                                     void* stream);
 
+/* ------------------------------------------------------------------ router: compact picks */
+
+/*
+ * Routing from the indices of a top-k instead of a [cell, path] mask (no counterpart in the
+ * reference, whose routers make the mask of them: python/brt/router/protocol/topk.py:26-31).
+ *
+ * brt_order_picks: picks[pick_total] (int32, or int64 when picks_are_64bit != 0), the picks of a
+ * cell next to each other -> places[pick_total], the row of each pick in a buffer of pick_total
+ * rows sorted by path (stable), and loads[path_num].  The same path may be picked twice.  A pick
+ * outside [0, path_num) goes nowhere: it is sorted behind the last path, and its place is
+ * -2 - row, naming the row at the end that stays empty for it.
+ * path_num <= 1024; scratch: brt_pick_order_scratch_bytes (0 for few picks), 4-byte aligned.
+ */
+BRT_API size_t brt_pick_order_scratch_bytes(int64_t pick_total, int path_num);
+BRT_API int brt_order_picks(const void* picks, int picks_are_64bit, int64_t pick_total,
+                            int path_num, int32_t* places, int32_t* loads, void* scratch,
+                            size_t scratch_bytes, void* stream);
+
+/*
+ * Rows over the places [cell_num, pick_num] of brt_order_picks; a buffer of rows has
+ * cell_num * pick_num of them.  Places p >= 0 are rows, p <= -2 an empty row -2 - p, -1 nothing
+ * at all; places outside the buffer are skipped.
+ *
+ * brt_sort_cells      rows[places[t, j]] = cells[t], zeros in the empty rows.
+ * brt_sort_cells_fp8  the same rows as brt_quantize_rows would make them; cell_size % 16 == 0,
+ *                     both arrays 16-byte aligned.
+ * brt_unsort_cells    cells[t] = sum over j of gates[t, j] * rows[places[t, j]] in fp32, in the
+ *                     order of j, rounded once (without gates: the plain sum, which is also the
+ *                     gradient of brt_sort_cells).  gates: fp32 or dtype, or null.
+ * brt_unsort_cells_backward  row_grads[places[t, j]] = gates[t, j] * cell_grads[t], zeros in the
+ *                     empty rows; gate_grads[t, j] (of gates_dtype) = <cell_grads[t],
+ *                     rows[places[t, j]]>, 0 for picks that go nowhere.  Either may be null
+ *                     (rows may be without gate_grads).
+ */
+BRT_API int brt_sort_cells(const void* cells, const int32_t* places, void* rows, int64_t cell_num,
+                           int pick_num, int64_t cell_size, int dtype, void* stream);
+BRT_API int brt_sort_cells_fp8(const void* cells, const int32_t* places, void* codes,
+                               float* scales, int64_t cell_num, int pick_num, int64_t cell_size,
+                               int dtype, void* stream);
+BRT_API int brt_unsort_cells(const void* rows, const int32_t* places, const void* gates,
+                             void* cells, int64_t cell_num, int pick_num, int64_t cell_size,
+                             int dtype, int gates_dtype, void* stream);
+BRT_API int brt_unsort_cells_backward(const void* cell_grads, const void* rows,
+                                      const int32_t* places, const void* gates, void* row_grads,
+                                      void* gate_grads, int64_t cell_num, int pick_num,
+                                      int64_t cell_size, int dtype, int gates_dtype,
+                                      void* stream);
+
+/* ------------------------------------------------------------------ experts: 8-bit products */
+
+/*
+ * 8-bit floating point (e4m3) with an fp32 scale for each block of 128 values, value = code *
+ * scale: scale = max(max |x|, 2^-100) / 448, code = e4m3(x * (448 / max(max |x|, 2^-100))).  No
+ * counterpart in the reference.  dtype: of the values; features are multiples of 16, arrays
+ * 16-byte aligned.
+ *
+ * brt_quantize_rows            rows [row_num, width] -> codes [row_num, width], scales
+ *                              [ceil(width / 128), row_num] (a block's scales of all rows lie
+ *                              together).
+ * brt_quantize_expert_weights  weights [path_num, out_features, in_features], a scale for each
+ *                              128 x 128 -> codes of that shape and scales [path_num,
+ *                              ceil(out / 128), ceil(in / 128)]; transposed != 0: both with in
+ *                              and out exchanged, as the product of the backward pass takes them.
+ */
+BRT_API int brt_quantize_rows(const void* rows, void* codes, float* scales, int64_t row_num,
+                              int64_t width, int dtype, void* stream);
+BRT_API int brt_quantize_expert_weights(const void* weights, void* codes, float* scales,
+                                        int path_num, int64_t in_features, int64_t out_features,
+                                        int transposed, int dtype, void* stream);
+
+/*
+ * brt_grouped_expert_gemm over such codes:
+ *   out[r, n] = act(sum over b of row_scales[r, b] * weight_scales[e, n / 128, b]
+ *                   * sum over k in block b of rows[r, k] * weights[e, n, k])
+ * with fp32 sums and bf16 out.  row_scales: element (r, b) at r * scale_row_stride + b *
+ * scale_block_stride.  Everything else as there; in_features % 16 == 0 and out_features % 16 == 0.
+ * zero_unused != 0 writes zeros to the rows of `out` that belong to no expert.
+ */
+BRT_API int brt_grouped_expert_gemm_fp8(const void* rows, const float* row_scales,
+                                        int64_t scale_row_stride, int64_t scale_block_stride,
+                                        const void* weights, const float* weight_scales,
+                                        void* out, const int32_t* loads, int path_num,
+                                        int64_t total_rows, int32_t max_path_load,
+                                        int64_t in_features, int64_t out_features, int relu,
+                                        int zero_unused, void* error_word, void* stream);
+
+/*
+ * The gradient of the experts' weights (no counterpart in the reference):
+ *   out[e, n, k] = sum over the rows r of expert e of grads[r, n] * rows[r, k]
+ * grads [total_rows, out_features] and rows [total_rows, in_features] bf16, laid out as for
+ * brt_grouped_expert_gemm; out [path_num, out_features, in_features] fp32 or bf16 (out_dtype), all
+ * of it written, zeros for experts without rows.  Rows that belong to no expert are not looked at.
+ */
+BRT_API int brt_grouped_expert_weight_grad(const void* grads, const void* rows, void* out,
+                                           const int32_t* loads, int path_num, int64_t total_rows,
+                                           int32_t max_path_load, int64_t in_features,
+                                           int64_t out_features, int out_dtype, void* error_word,
+                                           void* stream);
+
 /* ------------------------------------------------------------------ distributed: rank reorder */
 
 /*
