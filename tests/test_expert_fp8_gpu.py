@@ -292,7 +292,7 @@ def test_layer_of_all_operators_and_its_gradients():
     want_grads = torch.autograd.grad(want, leaves, gy.double())
     X.check_status()
     for a, b in zip((got,) + got_grads, (want,) + want_grads):
-        off = (a.double() - b.double()).norm() / b.double().norm()
+        off = (a.detach().double() - b.detach().double()).norm() / b.detach().double().norm()
         # each product's operands are off by at most 2^-4 of a value (0.036 rms of it) and four
         # such roundings are behind the deepest gradient
         assert float(off) < 4 * 2 * 2.0 ** -4, float(off)
