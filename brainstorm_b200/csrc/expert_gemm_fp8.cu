@@ -31,7 +31,7 @@
 //              one-lane-per-thread reads take (shared memory already carries the TMA's writes
 //              and the MMA's reads at its full rate).  At the end: ReLU, bf16, stmatrix turned
 //              so that a row's 32 features are stored together;
-//   warp 2     multiplies the two scales of the next blocks into a ring in shared memory.
+//   warps 2-3  multiply the two scales of the next blocks into a ring in shared memory.
 // Every wait is bounded: after the limit the role records an error and leaves its loop, the
 // copies in flight are given time to land, the CTAs meet, free tensor memory and return.
 #include <cuda_fp8.h>
@@ -50,7 +50,8 @@ constexpr int kBoxSizes = 4;
 constexpr int kMmaK = 32;
 constexpr int kScaleSlots = 4;
 constexpr int kAccWarps = 8;
-constexpr int kScaleWarp = 2;
+constexpr int kFirstScaleWarp = 2;
+constexpr int kScaleWarps = 2;
 constexpr int kFirstAccWarp = 4;  // warps are given registers by fours
 constexpr int kThreads = 32 * (kFirstAccWarp + kAccWarps);
 // The block starts with 168 registers a thread.  The accumulators alone are 128 of an
@@ -214,7 +215,7 @@ expert_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w,
         mbar_init(&s.acc_empty[i], kAccWarps * kPair);
       }
       for (int i = 0; i < kScaleSlots; i++) {
-        mbar_init(&s.scale_full[i], 1);
+        mbar_init(&s.scale_full[i], kScaleWarps);
         mbar_init(&s.scale_empty[i], kAccWarps);
       }
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -286,42 +287,64 @@ expert_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w,
           }
         }
       }
-    } else if (warp == kScaleWarp) {
+    } else {
+      // two warps, half of a tile's columns each; the scales of the next kAhead blocks are on
+      // their way while those of the last ones are handed over
+      const int half = warp - kFirstScaleWarp;
+      constexpr int kAhead = 4;
+      constexpr int kPer = kBN / 2 / 32;
+      float r[kAhead][kPer], w[kAhead];
       int slot = 0;
       uint32_t phase = 0;
-      for (int t = group; t < total_tiles && !failed; t += groups) {
-        const TileAt at = tile_at(s.table, g.experts, g.m_tiles, t);
+      TileAt at;
+      const auto fetch = [&](int kb0) {
         const int feature_block = at.m_tile * kPair + (int)rank;
-        const float* const ws = g.weight_scales +
-            ((long long)at.expert * g.n_blocks + feature_block) * g.k_blocks;
         const bool some = feature_block < g.n_blocks;  // a pair's second CTA may have no features
+        const float* const ws = g.weight_scales +
+            ((long long)at.expert * g.n_blocks + (some ? feature_block : 0)) * g.k_blocks;
         const float* const rs =
             g.row_scales + ((long long)s.table.row_base[at.expert] + at.row0) * g.row_stride;
-        constexpr int kAhead = 2;  // blocks whose scales are fetched together
-        for (int kb0 = 0; kb0 < g.k_blocks && !failed; kb0 += kAhead) {
-          float r[kAhead][kBN / 32], w[kAhead];
-  #pragma unroll
-          for (int h = 0; h < kAhead; h++) {
-            const bool real = kb0 + h < g.k_blocks;
-            w[h] = some && real ? __ldg(ws + kb0 + h) : 0.f;
-  #pragma unroll
-            for (int i = 0; i < kBN / 32; i++) {
-              const int c = i * 32 + lane;
-              r[h][i] = real && c < at.rows
-                            ? __ldg(rs + c * g.row_stride + (kb0 + h) * g.block_stride) : 0.f;
-            }
+#pragma unroll
+        for (int h = 0; h < kAhead; h++) {
+          const bool real = kb0 + h < g.k_blocks;
+          w[h] = some && real ? __ldg(ws + kb0 + h) : 0.f;
+#pragma unroll
+          for (int i = 0; i < kPer; i++) {
+            const int c = half * (kBN / 2) + i * 32 + lane;
+            r[h][i] = real && c < at.rows
+                          ? __ldg(rs + c * g.row_stride + (kb0 + h) * g.block_stride) : 0.f;
           }
-  #pragma unroll
-          for (int h = 0; h < kAhead; h++) {
-            if (kb0 + h >= g.k_blocks) break;
-            if (!mbar_wait(&s.scale_empty[slot], phase ^ 1)) { failed = true; break; }
-  #pragma unroll
-            for (int i = 0; i < kBN / 32; i++)
-              s.scale[slot][scale_at(i * 32 + lane)] = r[h][i] * w[h];
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&s.scale_full[slot]);
-            if (++slot == kScaleSlots) { slot = 0; phase ^= 1; }
-          }
+        }
+      };
+      int t = group, kb0 = 0;
+      if (t < total_tiles) {
+        at = tile_at(s.table, g.experts, g.m_tiles, t);
+        fetch(0);
+      }
+      while (t < total_tiles && !failed) {
+        float scale[kAhead][kPer];
+#pragma unroll
+        for (int h = 0; h < kAhead; h++)
+#pragma unroll
+          for (int i = 0; i < kPer; i++) scale[h][i] = r[h][i] * w[h];
+        const int blocks = min(kAhead, g.k_blocks - kb0);
+        kb0 += kAhead;
+        if (kb0 >= g.k_blocks) {
+          kb0 = 0;
+          t += groups;
+          if (t < total_tiles) at = tile_at(s.table, g.experts, g.m_tiles, t);
+        }
+        if (t < total_tiles) fetch(kb0);
+#pragma unroll
+        for (int h = 0; h < kAhead; h++) {
+          if (h >= blocks) break;
+          if (!mbar_wait(&s.scale_empty[slot], phase ^ 1)) { failed = true; break; }
+#pragma unroll
+          for (int i = 0; i < kPer; i++)
+            s.scale[slot][scale_at(half * (kBN / 2) + i * 32 + lane)] = scale[h][i];
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s.scale_full[slot]);
+          if (++slot == kScaleSlots) { slot = 0; phase ^= 1; }
         }
       }
     }
@@ -375,7 +398,7 @@ expert_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w,
         __syncwarp();
         if (lane == 0) {
           if (rank == 0) mbar_arrive(&s.acc_empty[buf]);
-          else mbar_arrive_cluster(map_to_cta(&s.acc_empty[buf], 0));
+          else mbar_arrive_cluster_relaxed(map_to_cta(&s.acc_empty[buf], 0));
           mbar_arrive(&s.scale_empty[slot]);
         }
         if (++slot == kScaleSlots) { slot = 0; phase ^= 1; }

@@ -64,6 +64,13 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr)
                : "memory");
 }
+// The same for a thread that has written nothing the peer will read (it has only read tensor
+// memory, and its loads are complete): a release at cluster scope waits for all its earlier
+// accesses, which an accumulator handed back every few hundred cycles cannot afford.
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr)
+               : "memory");
+}
 // `bar` is a cluster address: with a pair, the copies of both CTAs count on the first one's.
 template <int kPair>
 __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, uint32_t bar,
