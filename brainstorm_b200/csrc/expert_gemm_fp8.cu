@@ -187,6 +187,22 @@ __device__ __forceinline__ TileAt tile_at(const ExpertTable& table, int experts,
   return at;
 }
 
+// Zeros in the rows of `out` that belong to no expert, a warp each.
+__device__ __forceinline__ void zero_unused_rows(const ExpertTable& table, const Fp8Args& g,
+                                                 int first, int step) {
+  const int lane = threadIdx.x & 31;
+  const int parts = g.max_path_load != 0 ? g.experts : 1;
+  for (int e = 0; e < parts; e++) {
+    const int last = g.max_path_load != 0 ? e : g.experts - 1;
+    const long long from = (long long)table.row_base[last] + table.load[last];
+    const long long until =
+        g.max_path_load != 0 && e + 1 < parts ? table.row_base[e + 1] : g.total_rows;
+    for (long long r = from + first; r < until; r += step)
+      for (long long n = lane * 8; n < g.N; n += 256)
+        *reinterpret_cast<uint4*>(g.out + r * g.N + n) = make_uint4(0u, 0u, 0u, 0u);
+  }
+}
+
 template <int kPair>
 __global__ void __launch_bounds__(kThreads, 1)
 expert_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w,
@@ -440,20 +456,9 @@ expert_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w,
         __syncwarp();
       }
     }
-    if (g.zero_unused) {  // rows that belong to no expert, a warp each
-      const int first = blockIdx.x * kAccWarps + warp - kFirstAccWarp;
-      const int step = gridDim.x * kAccWarps;
-      const int parts = g.max_path_load != 0 ? g.experts : 1;
-      for (int e = 0; e < parts; e++) {
-        const int last = g.max_path_load != 0 ? e : g.experts - 1;
-        const long long from = (long long)s.table.row_base[last] + s.table.load[last];
-        const long long until =
-            g.max_path_load != 0 && e + 1 < parts ? s.table.row_base[e + 1] : g.total_rows;
-        for (long long r = from + first; r < until; r += step)
-          for (long long n = lane * 8; n < g.N; n += 256)
-            *reinterpret_cast<uint4*>(g.out + r * g.N + n) = make_uint4(0u, 0u, 0u, 0u);
-      }
-    }
+    if (g.zero_unused)
+      zero_unused_rows(s.table, g, blockIdx.x * kAccWarps + warp - kFirstAccWarp,
+                       gridDim.x * kAccWarps);
   }
   if (failed) atomicExch(g.error, BRT_ERR_TIMEOUT);
   __syncwarp();  // the single-lane roles rejoin their warps before the barrier
@@ -464,32 +469,258 @@ expert_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w,
   if (warp == 1) tmem_free<kPair>(tmem);
 }
 
-template <int kPair>
-int launch_fp8(const CUtensorMap& map_w, const RowMaps& map_r, const Fp8Args& g, cudaStream_t st) {
-  const size_t smem = sizeof(Fp8Smem<kPair>) + 1024;
-  static_assert(sizeof(Fp8Smem<kPair>) + 1024 <= 232448, "shared memory of an SM");
-  static thread_local int configured_device = -1;
-  int dev = 0;
-  BRT_CUDA_TRY(cudaGetDevice(&dev));
-  if (configured_device != dev) {
-    BRT_CUDA_TRY(cudaFuncSetAttribute(expert_gemm_fp8_kernel<kPair>,
-                                      cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    configured_device = dev;
+// ---- many rows per expert: the rows are the M operand -------------------------------------
+//
+// A CTA pair computes 256 rows x 256 features, 128 rows (the lanes of tensor memory) in each CTA.
+// A thread then holds 128 features of ONE row, a scale block, and needs one scale per block of K,
+// which it multiplies itself from two global values fetched blocks ahead: no scale ring and no
+// shared-memory reads beside the MMA's.  The last tile of an expert is computed in full, so
+// this pays from some hundred rows per expert on.
+
+constexpr int kRowsStages = 6;
+constexpr int kRowsFew = 40, kRowsMany = 232;
+static_assert(128 * kRowsFew + 32 * kAccWarps * kRowsMany == kThreads * 168, "registers");
+constexpr int kRowsAsM = 512;  // rows per expert on average
+
+struct alignas(1024) Fp8RowsSmem {
+  unsigned char a[kRowsStages][kTileBytes];  // 128 rows
+  unsigned char b[kRowsStages][kTileBytes];  // 128 features: half of the pair's
+  unsigned char turn[kAccWarps][32 * 64];
+  uint64_t full[kRowsStages];
+  uint64_t empty[kRowsStages];
+  uint64_t acc_full[2];
+  uint64_t acc_empty[2];
+  uint32_t tmem_base;
+  ExpertTable table;
+};
+
+static_assert(sizeof(Fp8RowsSmem) + 1024 <= 232448 && sizeof(Fp8Smem<1>) + 1024 <= 232448 &&
+              sizeof(Fp8Smem<2>) + 1024 <= 232448, "shared memory of an SM");
+
+struct RowsTile {
+  int expert, n_tile;
+  int row0, rows;  // within the expert
+};
+__device__ __forceinline__ RowsTile rows_tile(const ExpertTable& table, int experts, int n_tiles,
+                                              int t) {
+  RowsTile at;
+  at.expert = expert_of_tile(table, experts, t);
+  const int local = t - table.first_tile[at.expert];
+  const int part = local / n_tiles;
+  at.n_tile = local - part * n_tiles;
+  at.row0 = part * 2 * kBM;
+  at.rows = min(2 * kBM, table.load[at.expert] - at.row0);
+  return at;
+}
+
+__global__ void __launch_bounds__(kThreads, 1)
+expert_gemm_fp8_rows_kernel(const __grid_constant__ CUtensorMap map_w,
+                            const __grid_constant__ CUtensorMap map_r, const Fp8Args g) {
+  extern __shared__ __align__(1024) unsigned char s_raw[];
+  Fp8RowsSmem& s = *reinterpret_cast<Fp8RowsSmem*>(
+      (reinterpret_cast<uintptr_t>(s_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const int group = blockIdx.x / 2;
+  const int groups = gridDim.x / 2;
+  const int n_tiles = g.m_tiles;
+
+  if (warp == 0) {
+    fill_expert_table(s.table, g.loads, g.experts, g.max_path_load, g.total_rows,
+                      [n_tiles](int load) { return (load + 2 * kBM - 1) / (2 * kBM) * n_tiles; });
+    if (lane == 0) {
+      for (int i = 0; i < kRowsStages; i++) {
+        mbar_init(&s.full[i], 1);
+        mbar_init(&s.empty[i], 1);
+      }
+      for (int i = 0; i < 2; i++) {
+        mbar_init(&s.acc_full[i], 1);
+        mbar_init(&s.acc_empty[i], kAccWarps * 2);
+      }
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
   }
+  if (warp == 1) tmem_alloc<2>(&s.tmem_base);
+  tcgen05_before_sync();
+  __syncthreads();
+  group_sync<2>();
+  tcgen05_after_sync();
+  const uint32_t tmem = s.tmem_base;
+  const int total_tiles = s.table.first_tile[g.experts];
+  bool failed = false;
+
+  if (warp < kFirstAccWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRowsFew));
+    if (warp == 0) {
+      if (lane == 0) {
+        int slot = 0;
+        uint32_t phase = 0;
+        for (int t = group; t < total_tiles && !failed; t += groups) {
+          const RowsTile at = rows_tile(s.table, g.experts, n_tiles, t);
+          const int row0 = s.table.row_base[at.expert] + at.row0 + (int)rank * kBM;
+          const int feature0 = (at.n_tile * 2 + (int)rank) * kBM;
+          for (int kb = 0; kb < g.k_blocks; kb++) {
+            if (!mbar_wait(&s.empty[slot], phase ^ 1)) { failed = true; break; }
+            if (rank == 0) mbar_expect_tx(&s.full[slot], 4 * kTileBytes);
+            const uint32_t bar = map_to_cta(&s.full[slot], 0);
+            tma_load_2d<2>(s.a[slot], &map_r, bar, kb * kBK, row0);
+            tma_load_3d<2>(s.b[slot], &map_w, bar, kb * kBK, feature0, at.expert);
+            if (++slot == kRowsStages) { slot = 0; phase ^= 1; }
+          }
+        }
+        // copies still in flight land before the CTA's shared memory is given back
+        if (failed)
+          for (int i = 0; i < 1024; i++) __nanosleep(1000);
+      }
+    } else if (warp == 1 && lane == 0 && rank == 0) {
+      int slot = 0, buf = 0;
+      uint32_t phase = 0, buf_phase = 0;
+      const uint32_t idesc = fp8_idesc<2>(2 * kBM);
+      for (int t = group; t < total_tiles && !failed; t += groups) {
+        for (int kb = 0; kb < g.k_blocks; kb++) {
+          if (!mbar_wait(&s.acc_empty[buf], buf_phase ^ 1) || !mbar_wait(&s.full[slot], phase)) {
+            failed = true;
+            break;
+          }
+          tcgen05_after_sync();
+          const uint64_t da = umma_desc(s.a[slot]);
+          const uint64_t db = umma_desc(s.b[slot]);
+          const uint32_t d = tmem + (uint32_t)buf * kBN;
+#pragma unroll
+          for (int k = 0; k < kBK / kMmaK; k++) mma_fp8<2>(d, da + 2 * k, db + 2 * k, idesc, k != 0);
+          umma_commit<2>(&s.empty[slot]);
+          umma_commit<2>(&s.acc_full[buf]);
+          if (++slot == kRowsStages) { slot = 0; phase ^= 1; }
+          buf ^= 1;
+          if (buf == 0) buf_phase ^= 1;
+        }
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRowsMany));
+    const int quarter = warp & 3;
+    const int half = (warp - kFirstAccWarp) / 4;  // of the tile's features: one scale block
+    unsigned char* const turn = s.turn[warp - kFirstAccWarp];
+    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * kBM);
+    int buf = 0;
+    uint32_t buf_phase = 0;
+    constexpr int kAhead = 4;  // blocks whose scales are on their way
+    for (int t = group; t < total_tiles && !failed; t += groups) {
+      const RowsTile at = rows_tile(s.table, g.experts, n_tiles, t);
+      const int row0 = (int)rank * kBM + quarter * 32;  // of the tile
+      const long long first = (long long)s.table.row_base[at.expert] + at.row0 + row0;
+      const int feature_block = at.n_tile * 2 + half;
+      const bool some = feature_block < g.n_blocks && row0 + lane < at.rows;
+      const float* const rs = g.row_scales + (some ? (first + lane) * g.row_stride : 0);
+      const float* const ws = g.weight_scales +
+          (some ? ((long long)at.expert * g.n_blocks + feature_block) * g.k_blocks : 0);
+      float r[kAhead], w[kAhead];
+#pragma unroll
+      for (int h = 0; h < kAhead; h++) {
+        r[h] = some && h < g.k_blocks ? __ldg(rs + h * g.block_stride) : 0.f;
+        w[h] = some && h < g.k_blocks ? __ldg(ws + h) : 0.f;
+      }
+      float acc[kBM];
+#pragma unroll
+      for (int i = 0; i < kBM; i++) acc[i] = 0.f;
+      for (int kb0 = 0; kb0 < g.k_blocks && !failed; kb0 += kAhead) {
+#pragma unroll
+        for (int h = 0; h < kAhead; h++) {
+          const int kb = kb0 + h;
+          if (kb >= g.k_blocks) break;
+          const float scale = r[h] * w[h];
+          if (some && kb + kAhead < g.k_blocks) {
+            r[h] = __ldg(rs + (kb + kAhead) * g.block_stride);
+            w[h] = __ldg(ws + kb + kAhead);
+          }
+          if (!mbar_wait(&s.acc_full[buf], buf_phase)) { failed = true; break; }
+          tcgen05_after_sync();
+          const uint32_t from = lanes + (uint32_t)(buf * kBN);
+          uint32_t v[2][32];
+          tmem_load_32(from, v[0]);
+#pragma unroll
+          for (int c = 0; c < 4; c++) {
+            tmem_load_wait();
+            if (c < 3) tmem_load_32(from + (c + 1) * 32, v[(c + 1) & 1]);
+            if (c == 3) {  // everything is in registers: the next block may be multiplied into it
+              tcgen05_before_sync();
+              __syncwarp();
+              if (lane == 0) {
+                if (rank == 0) mbar_arrive(&s.acc_empty[buf]);
+                else mbar_arrive_cluster_relaxed(map_to_cta(&s.acc_empty[buf], 0));
+              }
+            }
+#pragma unroll
+            for (int i = 0; i < 32; i++)
+              acc[c * 32 + i] = fmaf(__uint_as_float(v[c & 1][i]), scale, acc[c * 32 + i]);
+          }
+          buf ^= 1;
+          if (buf == 0) buf_phase ^= 1;
+        }
+      }
+      if (failed) break;
+      const int rows = at.rows - row0;
+      const int feature = feature_block * kBM + (lane & 3) * 8;
+      __nv_bfloat16* const out = g.out + first * g.N + feature;
+#pragma unroll
+      for (int c = 0; c < 4; c++) {
+        uint32_t packed[16];
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+          float lo = acc[c * 32 + 2 * i], hi = acc[c * 32 + 2 * i + 1];
+          if (g.relu) { lo = fmaxf(lo, 0.f); hi = fmaxf(hi, 0.f); }
+          const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
+          memcpy(&packed[i], &p, 4);
+        }
+        // 64 bytes per row, its four pieces exchanged by the row's number: no bank conflicts
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          *reinterpret_cast<uint4*>(turn + lane * 64 + ((i ^ (lane >> 1)) & 3) * 16) =
+              make_uint4(packed[4 * i], packed[4 * i + 1], packed[4 * i + 2], packed[4 * i + 3]);
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const int row = i * 8 + (lane >> 2);
+          if (row < rows && feature + c * 32 < g.N)
+            *reinterpret_cast<uint4*>(out + (long long)row * g.N + c * 32) =
+                *reinterpret_cast<const uint4*>(turn + row * 64 + ((lane ^ (row >> 1)) & 3) * 16);
+        }
+        __syncwarp();
+      }
+    }
+    if (g.zero_unused)
+      zero_unused_rows(s.table, g, blockIdx.x * kAccWarps + warp - kFirstAccWarp,
+                       gridDim.x * kAccWarps);
+  }
+  if (failed) atomicExch(g.error, BRT_ERR_TIMEOUT);
+  __syncwarp();
+
+  tcgen05_before_sync();
+  group_sync<2>();
+  tcgen05_after_sync();
+  if (warp == 1) tmem_free<2>(tmem);
+}
+
+template <typename Kernel, typename MapR>
+int launch_fp8(Kernel kernel, int pair, size_t smem, const CUtensorMap& map_w, const MapR& map_r,
+               const Fp8Args& g, cudaStream_t st) {
+  BRT_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    (int)smem));
   cudaLaunchAttribute cluster;
   cluster.id = cudaLaunchAttributeClusterDimension;
-  cluster.val.clusterDim.x = kPair;
+  cluster.val.clusterDim.x = pair;
   cluster.val.clusterDim.y = 1;
   cluster.val.clusterDim.z = 1;
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3((unsigned)(sm_count() / kPair * kPair));
+  config.gridDim = dim3((unsigned)(sm_count() / pair * pair));
   config.blockDim = dim3(kThreads);
   config.dynamicSmemBytes = smem;
   config.stream = st;
   config.attrs = &cluster;
   config.numAttrs = 1;
   const KernelTimer timer("expert_gemm_fp8_kernel", st);
-  BRT_CUDA_TRY(cudaLaunchKernelEx(&config, expert_gemm_fp8_kernel<kPair>, map_w, map_r, g));
+  BRT_CUDA_TRY(cudaLaunchKernelEx(&config, kernel, map_w, map_r, g));
   note_launch();
   return BRT_OK;
 }
@@ -530,6 +761,8 @@ BRT_API int brt_grouped_expert_gemm_fp8(const void* rows, const float* row_scale
   // a pair of CTAs computes two blocks of 128 features; single CTAs where an odd number would
   // leave half a pair idle for a large share of the work
   const int pair = n_blocks % 2 == 0 || n_blocks > 6 ? 2 : 1;
+  const int64_t mean_rows = max_path_load != 0 ? max_path_load : total_rows / path_num;
+  const bool rows_as_m = pair == 2 && mean_rows >= kRowsAsM;
   const int m_tiles = (n_blocks + pair - 1) / pair;
   BRT_REQUIRE((total_rows / kBN + path_num) * (int64_t)m_tiles < (1LL << 31) - 1024,
               "more tiles than 32 bits count");
@@ -584,7 +817,12 @@ BRT_API int brt_grouped_expert_gemm_fp8(const void* rows, const float* row_scale
   g.relu = relu != 0;
   g.zero_unused = zero_unused != 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return pair == 2 ? launch_fp8<2>(map_w, map_r, g, st) : launch_fp8<1>(map_w, map_r, g, st);
+  if (rows_as_m)
+    return launch_fp8(expert_gemm_fp8_rows_kernel, 2, sizeof(Fp8RowsSmem) + 1024, map_w,
+                      map_r.box[kBoxSizes - 1], g, st);
+  if (pair == 2)
+    return launch_fp8(expert_gemm_fp8_kernel<2>, 2, sizeof(Fp8Smem<2>) + 1024, map_w, map_r, g, st);
+  return launch_fp8(expert_gemm_fp8_kernel<1>, 1, sizeof(Fp8Smem<1>) + 1024, map_w, map_r, g, st);
 }
 
 }  // extern "C"
