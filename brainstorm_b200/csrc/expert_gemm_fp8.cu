@@ -248,36 +248,39 @@ expert_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w,
   if (warp < kFirstAccWarp) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegisters));
     if (warp == 0) {
-      if (lane == 0) {
-        int slot = 0;
-        uint32_t phase = 0;
-        for (int t = group; t < total_tiles && !failed; t += groups) {
-          const TileAt at = tile_at(s.table, g.experts, g.m_tiles, t);
-          const int half = at.width / kPair;  // rows this CTA stages
-          const int boxes = half > kBoxSizes * kBoxStep ? 2 : 1;
-          const int size = (half / boxes + kBoxStep - 1) / kBoxStep;
-          const int box_rows = size * kBoxStep;
-          const CUtensorMap* const map_box = &map_r.box[size - 1];
-          const int row0 = s.table.row_base[at.expert] + at.row0 + (int)rank * half;
-          const int feature0 = (at.m_tile * kPair + (int)rank) * kBM;
-          const uint32_t bytes = kPair * (kTileBytes + (uint32_t)(boxes * box_rows) * kRowBytes);
-          for (int kb = 0; kb < g.k_blocks; kb++) {
-            if (!mbar_wait(&s.empty[slot], phase ^ 1)) { failed = true; break; }
+      int slot = 0;
+      uint32_t phase = 0;
+      for (int t = group; t < total_tiles && !failed; t += groups) {
+        const TileAt at = tile_at(s.table, g.experts, g.m_tiles, t);
+        const int half = at.width / kPair;  // rows this CTA stages
+        const int boxes = half > kBoxSizes * kBoxStep ? 2 : 1;
+        const int size = (half / boxes + kBoxStep - 1) / kBoxStep;
+        const int box_rows = size * kBoxStep;
+        const CUtensorMap* const map_box = &map_r.box[size - 1];
+        const int row0 = s.table.row_base[at.expert] + at.row0 + (int)rank * half;
+        const int feature0 = (at.m_tile * kPair + (int)rank) * kBM;
+        const uint32_t bytes = kPair * (kTileBytes + (uint32_t)(boxes * box_rows) * kRowBytes);
+        for (int kb = 0; kb < g.k_blocks; kb++) {
+          if (!mbar_wait(&s.empty[slot], phase ^ 1)) { failed = true; break; }
+          if (elect_one()) {
             if (rank == 0) mbar_expect_tx(&s.full[slot], bytes);
-            const uint32_t bar = kPair == 2 ? map_to_cta(&s.full[slot], 0) : smem_u32(&s.full[slot]);
+            const uint32_t bar =
+                kPair == 2 ? map_to_cta(&s.full[slot], 0) : smem_u32(&s.full[slot]);
             tma_load_3d<kPair>(s.a[slot], &map_w, bar, kb * kBK, feature0, at.expert);
-            for (int b = 0; b < boxes; b++)
-              tma_load_2d<kPair>(s.b[slot] + b * box_rows * kRowBytes, map_box, bar, kb * kBK,
-                                 row0 + b * box_rows);
-            if (++slot == kRing) { slot = 0; phase ^= 1; }
+            tma_load_2d<kPair>(s.b[slot], map_box, bar, kb * kBK, row0);
+            if (kPair == 1 && boxes == 2)
+              tma_load_2d<kPair>(s.b[slot] + box_rows * kRowBytes, map_box, bar, kb * kBK,
+                                 row0 + box_rows);
           }
+          __syncwarp();
+          if (++slot == kRing) { slot = 0; phase ^= 1; }
         }
-        // copies still in flight land before the CTA's shared memory is given back
-        if (failed)
-          for (int i = 0; i < 1024; i++) __nanosleep(1000);
       }
+      // copies still in flight land before the CTA's shared memory is given back
+      if (failed)
+        for (int i = 0; i < 1024; i++) __nanosleep(1000);
     } else if (warp == 1) {
-      if (lane == 0 && rank == 0) {
+      if (rank == 0) {
         int slot = 0, buf = 0;
         uint32_t phase = 0, buf_phase = 0;
         for (int t = group; t < total_tiles && !failed; t += groups) {
@@ -289,14 +292,17 @@ expert_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w,
               break;
             }
             tcgen05_after_sync();
-            const uint64_t da = umma_desc(s.a[slot]);
-            const uint64_t db = umma_desc(s.b[slot]);
-            const uint32_t d = tmem + (uint32_t)buf * kBN;
-  #pragma unroll
-            for (int k = 0; k < kBK / kMmaK; k++)  // 32 bytes further along the swizzled row each
-              mma_fp8<kPair>(d, da + 2 * k, db + 2 * k, idesc, k != 0);
-            umma_commit<kPair>(&s.empty[slot]);
-            umma_commit<kPair>(&s.acc_full[buf]);
+            if (elect_one()) {
+              const uint64_t da = umma_desc(s.a[slot]);
+              const uint64_t db = umma_desc(s.b[slot]);
+              const uint32_t d = tmem + (uint32_t)buf * kBN;
+#pragma unroll
+              for (int k = 0; k < kBK / kMmaK; k++)  // 32 bytes further along the swizzled row
+                mma_fp8<kPair>(d, da + 2 * k, db + 2 * k, idesc, k != 0);
+              umma_commit<kPair>(&s.empty[slot]);
+              umma_commit<kPair>(&s.acc_full[buf]);
+            }
+            __syncwarp();
             if (++slot == kRing) { slot = 0; phase ^= 1; }
             buf ^= 1;
             if (buf == 0) buf_phase ^= 1;
@@ -553,27 +559,28 @@ expert_gemm_fp8_rows_kernel(const __grid_constant__ CUtensorMap map_w,
   if (warp < kFirstAccWarp) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRowsFew));
     if (warp == 0) {
-      if (lane == 0) {
-        int slot = 0;
-        uint32_t phase = 0;
-        for (int t = group; t < total_tiles && !failed; t += groups) {
-          const RowsTile at = rows_tile(s.table, g.experts, n_tiles, t);
-          const int row0 = s.table.row_base[at.expert] + at.row0 + (int)rank * kBM;
-          const int feature0 = (at.n_tile * 2 + (int)rank) * kBM;
-          for (int kb = 0; kb < g.k_blocks; kb++) {
-            if (!mbar_wait(&s.empty[slot], phase ^ 1)) { failed = true; break; }
+      int slot = 0;
+      uint32_t phase = 0;
+      for (int t = group; t < total_tiles && !failed; t += groups) {
+        const RowsTile at = rows_tile(s.table, g.experts, n_tiles, t);
+        const int row0 = s.table.row_base[at.expert] + at.row0 + (int)rank * kBM;
+        const int feature0 = (at.n_tile * 2 + (int)rank) * kBM;
+        for (int kb = 0; kb < g.k_blocks; kb++) {
+          if (!mbar_wait(&s.empty[slot], phase ^ 1)) { failed = true; break; }
+          if (elect_one()) {
             if (rank == 0) mbar_expect_tx(&s.full[slot], 4 * kTileBytes);
             const uint32_t bar = map_to_cta(&s.full[slot], 0);
             tma_load_2d<2>(s.a[slot], &map_r, bar, kb * kBK, row0);
             tma_load_3d<2>(s.b[slot], &map_w, bar, kb * kBK, feature0, at.expert);
-            if (++slot == kRowsStages) { slot = 0; phase ^= 1; }
           }
+          __syncwarp();
+          if (++slot == kRowsStages) { slot = 0; phase ^= 1; }
         }
-        // copies still in flight land before the CTA's shared memory is given back
-        if (failed)
-          for (int i = 0; i < 1024; i++) __nanosleep(1000);
       }
-    } else if (warp == 1 && lane == 0 && rank == 0) {
+      // copies still in flight land before the CTA's shared memory is given back
+      if (failed)
+        for (int i = 0; i < 1024; i++) __nanosleep(1000);
+    } else if (warp == 1 && rank == 0) {
       int slot = 0, buf = 0;
       uint32_t phase = 0, buf_phase = 0;
       const uint32_t idesc = fp8_idesc<2>(2 * kBM);
@@ -584,13 +591,17 @@ expert_gemm_fp8_rows_kernel(const __grid_constant__ CUtensorMap map_w,
             break;
           }
           tcgen05_after_sync();
-          const uint64_t da = umma_desc(s.a[slot]);
-          const uint64_t db = umma_desc(s.b[slot]);
-          const uint32_t d = tmem + (uint32_t)buf * kBN;
+          if (elect_one()) {
+            const uint64_t da = umma_desc(s.a[slot]);
+            const uint64_t db = umma_desc(s.b[slot]);
+            const uint32_t d = tmem + (uint32_t)buf * kBN;
 #pragma unroll
-          for (int k = 0; k < kBK / kMmaK; k++) mma_fp8<2>(d, da + 2 * k, db + 2 * k, idesc, k != 0);
-          umma_commit<2>(&s.empty[slot]);
-          umma_commit<2>(&s.acc_full[buf]);
+            for (int k = 0; k < kBK / kMmaK; k++)
+              mma_fp8<2>(d, da + 2 * k, db + 2 * k, idesc, k != 0);
+            umma_commit<2>(&s.empty[slot]);
+            umma_commit<2>(&s.acc_full[buf]);
+          }
+          __syncwarp();
           if (++slot == kRowsStages) { slot = 0; phase ^= 1; }
           buf ^= 1;
           if (buf == 0) buf_phase ^= 1;

@@ -30,6 +30,21 @@ __device__ __forceinline__ unsigned long long now_ns() {
   asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
   return t;
 }
+// True in one lane of the (whole) warp.  The loops around TMA and MMA instructions are run by all
+// lanes, and only the instructions themselves by the elected one: their operands then stay in
+// uniform registers.  A loop that one lane runs alone issued the four MMAs of a k-block every
+// 1080 cycles where the tensor cores need 512.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t yes;
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "elect.sync _|p, 0xffffffff;\n"
+      "selp.u32 %0, 1, 0, p;\n"
+      "}\n"
+      : "=r"(yes));
+  return yes != 0;
+}
 // Bounded wait for the phase with the given parity; false when the limit ran out.
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity) {
   const uint32_t addr = smem_u32(bar);
