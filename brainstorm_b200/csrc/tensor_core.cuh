@@ -86,6 +86,11 @@ __device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_add
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr)
                : "memory");
 }
+// An arrival of this thread as soon as its cp.async copies so far have landed (the barrier counts
+// it among its expected arrivals).
+__device__ __forceinline__ void mbar_arrive_copied(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
 // `bar` is a cluster address: with a pair, the copies of both CTAs count on the first one's.
 template <int kPair>
 __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, uint32_t bar,
