@@ -150,17 +150,17 @@ expert_wgrad_kernel(const __grid_constant__ CUtensorMap map_g,
   bool failed = false;
 
   if (warp == 0) {
-    if (lane == 0) {
-      int slot = 0;
-      uint32_t phase = 0;
-      const int b_boxes = (half + kBoxFeatures - 1) / kBoxFeatures;
-      const uint32_t bytes = (uint32_t)(kABoxes + b_boxes) * kBoxBytes;
-      for (int t = group; t < total_tiles && !failed; t += groups) {
-        const WgradTile at = wgrad_tile<kPair>(s.table, g, t);
-        const int n0 = at.n0 + (int)rank * kBM;
-        const int k0 = at.k0 + (int)rank * half;
-        for (int i = 0; i < at.blocks; i++) {
-          if (!mbar_wait(&s.empty[slot], phase ^ 1)) { failed = true; break; }
+    int slot = 0;
+    uint32_t phase = 0;
+    const int b_boxes = (half + kBoxFeatures - 1) / kBoxFeatures;
+    const uint32_t bytes = (uint32_t)(kABoxes + b_boxes) * kBoxBytes;
+    for (int t = group; t < total_tiles && !failed; t += groups) {
+      const WgradTile at = wgrad_tile<kPair>(s.table, g, t);
+      const int n0 = at.n0 + (int)rank * kBM;
+      const int k0 = at.k0 + (int)rank * half;
+      for (int i = 0; i < at.blocks; i++) {
+        if (!mbar_wait(&s.empty[slot], phase ^ 1)) { failed = true; break; }
+        if (elect_one()) {
           uint32_t bar;
           if (at.load - i * kBR < kBR) {  // the expert ends here: warp 2 passes the slot on
             mbar_expect_tx(&s.tail[slot], bytes);
@@ -168,22 +168,27 @@ expert_wgrad_kernel(const __grid_constant__ CUtensorMap map_g,
           } else {
             bar = kPair == 2 ? map_to_cta(&s.full[slot], 0) : smem_u32(&s.full[slot]);
             if (rank == 0) mbar_expect_tx(&s.full[slot], kPair * bytes);
-            else mbar_arrive_cluster(bar);
+            else mbar_arrive_cluster_relaxed(bar);
           }
           const int row = at.row0 + i * kBR;
+#pragma unroll
           for (int b = 0; b < kABoxes; b++)
             tma_load_2d<kPair>(s.a[slot] + b * kBoxBytes, &map_g, bar, n0 + b * kBoxFeatures, row);
-          for (int b = 0; b < b_boxes; b++)
-            tma_load_2d<kPair>(s.b[slot] + b * kBoxBytes, &map_r, bar, k0 + b * kBoxFeatures, row);
-          if (++slot == kRing) { slot = 0; phase ^= 1; }
+#pragma unroll
+          for (int b = 0; b < kBBoxes<kPair>; b++)
+            if (b < b_boxes)
+              tma_load_2d<kPair>(s.b[slot] + b * kBoxBytes, &map_r, bar, k0 + b * kBoxFeatures,
+                                 row);
         }
+        __syncwarp();
+        if (++slot == kRing) { slot = 0; phase ^= 1; }
       }
-      // copies still in flight land before the CTA's shared memory is given back
-      if (failed)
-        for (int i = 0; i < 1024; i++) __nanosleep(1000);
     }
+    // copies still in flight land before the CTA's shared memory is given back
+    if (failed)
+      for (int i = 0; i < 1024; i++) __nanosleep(1000);
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
       int slot = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       const uint32_t idesc = wgrad_idesc<kPair>(g.width);
@@ -196,17 +201,20 @@ expert_wgrad_kernel(const __grid_constant__ CUtensorMap map_g,
         for (int i = 0; i < at.blocks; i++) {
           if (!mbar_wait(&s.full[slot], phase)) { failed = true; break; }
           tcgen05_after_sync();
-          const uint64_t da = wgrad_desc(s.a[slot]);
-          const uint64_t db = wgrad_desc(s.b[slot]);
           const int rows = at.load - i * kBR;
-          const int steps = rows >= kBR ? kBR / kMmaK : (rows + kMmaK - 1) / kMmaK;
-          for (int k = 0; k < steps; k++)  // 16 rows of 128 bytes further each
-            umma_bf16<kPair>(d, da + 128 * k, db + 128 * k, idesc, (i | k) != 0);
-          umma_commit<kPair>(&s.empty[slot]);
+          if (elect_one()) {
+            const uint64_t da = wgrad_desc(s.a[slot]);
+            const uint64_t db = wgrad_desc(s.b[slot]);
+#pragma unroll
+            for (int k = 0; k < kBR / kMmaK; k++)  // 16 rows of 128 bytes further each
+              if (k * kMmaK < rows)
+                umma_bf16<kPair>(d, da + 128 * k, db + 128 * k, idesc, (i | k) != 0);
+            umma_commit<kPair>(&s.empty[slot]);
+            if (i + 1 == at.blocks) umma_commit<kPair>(&s.acc_full[acc]);
+          }
+          __syncwarp();
           if (++slot == kRing) { slot = 0; phase ^= 1; }
         }
-        if (failed) break;
-        umma_commit<kPair>(&s.acc_full[acc]);
         if (++acc == 2) { acc = 0; acc_phase ^= 1; }
       }
     }
