@@ -14,10 +14,18 @@
 // rows behind them are another expert's or none at all: of the last slot only ceil(rows / 16) MMA
 // steps run, and warp 2 first writes zeros over what the last step would read beyond the end in
 // both operands (zeros in one would not do: the other may hold NaN or infinities).
-// Roles inside a CTA (256 threads): warp 0 TMA loads, warp 1 tensor memory and MMAs, warp 2 the
-// ends of experts, warps 4-7 epilogue (tensor memory -> registers -> 64 bytes of a row at a time),
-// under the MMAs of the next tile thanks to two accumulators.  Every wait is bounded as in the
-// other expert kernels.
+// Additions in tensor memory need not round to nearest, so their errors add up instead of
+// cancelling: after 1024 rows an accumulator is added to fp32 registers and begun anew (9001 rows in
+// 30 uneven experts, against 64 bits: 1.5e-6 without, 6.6e-7 with).
+// Roles inside a CTA (384 threads): warp 0 TMA loads, warp 1 tensor memory and MMAs, warp 2 the
+// ends of experts, warps 4-11 sums and output, four warps for each half of the tile's columns,
+// under the MMAs that follow thanks to two accumulators.  A thread holds up to 128 values of
+// one row of the output and stores whole sectors.  Every wait is bounded as in the other expert
+// kernels.
+//
+// What bounds it: the tensor pipe and shared memory together (65536 rows in 32 experts, 1024 x
+// 4096: 384 us, 1432 TFLOP/s, 0.88 of the rate measured for a bf16 product); with few rows per expert
+// writing the gradients.
 #include "expert_tiles.cuh"
 #include "tensor_core.cuh"
 
@@ -31,8 +39,12 @@ constexpr int kBoxFeatures = 64;
 constexpr uint32_t kBoxBytes = kBoxFeatures * kBR * 2;  // 8 KB
 constexpr int kABoxes = kBM / kBoxFeatures;
 constexpr int kMmaK = 16;
-constexpr int kFirstEpilogueWarp = 4;
-constexpr int kThreads = 256;
+constexpr int kFirstSumWarp = 4;  // warps are given registers by fours
+constexpr int kSumWarps = 8;
+constexpr int kThreads = 32 * (kFirstSumWarp + kSumWarps);
+constexpr int kFewRegisters = 88, kManyRegisters = 208;
+static_assert(128 * kFewRegisters + 32 * kSumWarps * kManyRegisters == kThreads * 168, "registers");
+constexpr int kChunk = 16;     // ring slots (1024 rows) per accumulator
 template <int kPair>
 constexpr int kStages = kPair == 2 ? 6 : 4;
 template <int kPair>
@@ -73,7 +85,6 @@ template <int kPair>
 struct alignas(1024) WgradSmem {
   unsigned char a[kStages<kPair>][kABoxes * kBoxBytes];
   unsigned char b[kStages<kPair>][kBBoxes<kPair> * kBoxBytes];
-  unsigned char turn[4][32 * 64];
   uint64_t full[kStages<kPair>];
   uint64_t empty[kStages<kPair>];
   uint64_t tail[kStages<kPair>];  // this CTA's bytes of a slot where an expert ends
@@ -104,9 +115,21 @@ __device__ __forceinline__ WgradTile wgrad_tile(const ExpertTable& table, const 
   return at;
 }
 
-// One 16-byte piece per lane of rows of 64 bytes, eight rows at a time.
-__device__ __forceinline__ uint4 turned_piece(const unsigned char* turn, int r, int lane) {
-  return *reinterpret_cast<const uint4*>(turn + r * 64 + ((lane ^ (r >> 1)) & 3) * 16);
+// 32 bytes by one thread: a whole sector.
+__device__ __forceinline__ void store_sector(void* p, const uint32_t (&r)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+// The empty statements keep the additions in front of the loads that follow (the compiler would
+// hold more columns in registers than there are).
+__device__ __forceinline__ void add_columns(float* sum, const uint32_t (&v)[32]) {
+#pragma unroll
+  for (int i = 0; i < 32; i++) sum[i] += __uint_as_float(v[i]);
+#pragma unroll
+  for (int i = 0; i < 32; i += 8)
+    asm volatile("" : "+f"(sum[i]), "+f"(sum[i + 1]), "+f"(sum[i + 2]), "+f"(sum[i + 3]),
+                      "+f"(sum[i + 4]), "+f"(sum[i + 5]), "+f"(sum[i + 6]), "+f"(sum[i + 7]));
 }
 
 template <int kPair, bool kFloatOut>
@@ -136,7 +159,7 @@ expert_wgrad_kernel(const __grid_constant__ CUtensorMap map_g,
       }
       for (int i = 0; i < 2; i++) {
         mbar_init(&s.acc_full[i], 1);
-        mbar_init(&s.acc_empty[i], 4 * kPair);
+        mbar_init(&s.acc_empty[i], kSumWarps * kPair);
       }
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -149,175 +172,161 @@ expert_wgrad_kernel(const __grid_constant__ CUtensorMap map_g,
   const uint32_t tmem = s.tmem_base;
   bool failed = false;
 
-  if (warp == 0) {
-    int slot = 0;
-    uint32_t phase = 0;
-    const int b_boxes = (half + kBoxFeatures - 1) / kBoxFeatures;
-    const uint32_t bytes = (uint32_t)(kABoxes + b_boxes) * kBoxBytes;
-    for (int t = group; t < total_tiles && !failed; t += groups) {
-      const WgradTile at = wgrad_tile<kPair>(s.table, g, t);
-      const int n0 = at.n0 + (int)rank * kBM;
-      const int k0 = at.k0 + (int)rank * half;
-      for (int i = 0; i < at.blocks; i++) {
-        if (!mbar_wait(&s.empty[slot], phase ^ 1)) { failed = true; break; }
-        if (elect_one()) {
-          uint32_t bar;
-          if (at.load - i * kBR < kBR) {  // the expert ends here: warp 2 passes the slot on
-            mbar_expect_tx(&s.tail[slot], bytes);
-            bar = kPair == 2 ? map_to_cta(&s.tail[slot], rank) : smem_u32(&s.tail[slot]);
-          } else {
-            bar = kPair == 2 ? map_to_cta(&s.full[slot], 0) : smem_u32(&s.full[slot]);
-            if (rank == 0) mbar_expect_tx(&s.full[slot], kPair * bytes);
-            else mbar_arrive_cluster_relaxed(bar);
-          }
-          const int row = at.row0 + i * kBR;
-#pragma unroll
-          for (int b = 0; b < kABoxes; b++)
-            tma_load_2d<kPair>(s.a[slot] + b * kBoxBytes, &map_g, bar, n0 + b * kBoxFeatures, row);
-#pragma unroll
-          for (int b = 0; b < kBBoxes<kPair>; b++)
-            if (b < b_boxes)
-              tma_load_2d<kPair>(s.b[slot] + b * kBoxBytes, &map_r, bar, k0 + b * kBoxFeatures,
-                                 row);
-        }
-        __syncwarp();
-        if (++slot == kRing) { slot = 0; phase ^= 1; }
-      }
-    }
-    // copies still in flight land before the CTA's shared memory is given back
-    if (failed)
-      for (int i = 0; i < 1024; i++) __nanosleep(1000);
-  } else if (warp == 1) {
-    if (rank == 0) {
-      int slot = 0, acc = 0;
-      uint32_t phase = 0, acc_phase = 0;
-      const uint32_t idesc = wgrad_idesc<kPair>(g.width);
+  if (warp < kFirstSumWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegisters));
+    if (warp == 0) {
+      int slot = 0;
+      uint32_t phase = 0;
+      const int b_boxes = (half + kBoxFeatures - 1) / kBoxFeatures;
+      const uint32_t bytes = (uint32_t)(kABoxes + b_boxes) * kBoxBytes;
       for (int t = group; t < total_tiles && !failed; t += groups) {
         const WgradTile at = wgrad_tile<kPair>(s.table, g, t);
-        if (at.blocks == 0) continue;
-        if (!mbar_wait(&s.acc_empty[acc], acc_phase ^ 1)) { failed = true; break; }
-        tcgen05_after_sync();
-        const uint32_t d = tmem + (uint32_t)acc * kBN;
+        const int n0 = at.n0 + (int)rank * kBM;
+        const int k0 = at.k0 + (int)rank * half;
         for (int i = 0; i < at.blocks; i++) {
-          if (!mbar_wait(&s.full[slot], phase)) { failed = true; break; }
-          tcgen05_after_sync();
-          const int rows = at.load - i * kBR;
+          if (!mbar_wait(&s.empty[slot], phase ^ 1)) { failed = true; break; }
           if (elect_one()) {
-            const uint64_t da = wgrad_desc(s.a[slot]);
-            const uint64_t db = wgrad_desc(s.b[slot]);
+            uint32_t bar;
+            if (at.load - i * kBR < kBR) {  // the expert ends here: warp 2 passes the slot on
+              mbar_expect_tx(&s.tail[slot], bytes);
+              bar = kPair == 2 ? map_to_cta(&s.tail[slot], rank) : smem_u32(&s.tail[slot]);
+            } else {
+              bar = kPair == 2 ? map_to_cta(&s.full[slot], 0) : smem_u32(&s.full[slot]);
+              if (rank == 0) mbar_expect_tx(&s.full[slot], kPair * bytes);
+              else mbar_arrive_cluster_relaxed(bar);
+            }
+            const int row = at.row0 + i * kBR;
 #pragma unroll
-            for (int k = 0; k < kBR / kMmaK; k++)  // 16 rows of 128 bytes further each
-              if (k * kMmaK < rows)
-                umma_bf16<kPair>(d, da + 128 * k, db + 128 * k, idesc, (i | k) != 0);
-            umma_commit<kPair>(&s.empty[slot]);
-            if (i + 1 == at.blocks) umma_commit<kPair>(&s.acc_full[acc]);
+            for (int b = 0; b < kABoxes; b++)
+              tma_load_2d<kPair>(s.a[slot] + b * kBoxBytes, &map_g, bar, n0 + b * kBoxFeatures, row);
+#pragma unroll
+            for (int b = 0; b < kBBoxes<kPair>; b++)
+              if (b < b_boxes)
+                tma_load_2d<kPair>(s.b[slot] + b * kBoxBytes, &map_r, bar, k0 + b * kBoxFeatures,
+                                   row);
           }
           __syncwarp();
           if (++slot == kRing) { slot = 0; phase ^= 1; }
         }
-        if (++acc == 2) { acc = 0; acc_phase ^= 1; }
+      }
+      // copies still in flight land before the CTA's shared memory is given back
+      if (failed)
+        for (int i = 0; i < 1024; i++) __nanosleep(1000);
+    } else if (warp == 1) {
+      if (rank == 0) {
+        int slot = 0, acc = 0;
+        uint32_t phase = 0, acc_phase = 0;
+        const uint32_t idesc = wgrad_idesc<kPair>(g.width);
+        for (int t = group; t < total_tiles && !failed; t += groups) {
+          const WgradTile at = wgrad_tile<kPair>(s.table, g, t);
+          for (int i = 0; i < at.blocks; i++) {
+            if ((i % kChunk == 0 && !mbar_wait(&s.acc_empty[acc], acc_phase ^ 1)) ||
+                !mbar_wait(&s.full[slot], phase)) {
+              failed = true;
+              break;
+            }
+            tcgen05_after_sync();
+            const int rows = at.load - i * kBR;
+            const bool last = i % kChunk == kChunk - 1 || i + 1 == at.blocks;
+            const uint32_t d = tmem + (uint32_t)acc * kBN;
+            if (elect_one()) {
+              const uint64_t da = wgrad_desc(s.a[slot]);
+              const uint64_t db = wgrad_desc(s.b[slot]);
+#pragma unroll
+              for (int k = 0; k < kBR / kMmaK; k++)  // 16 rows of 128 bytes further each
+                if (k * kMmaK < rows)
+                  umma_bf16<kPair>(d, da + 128 * k, db + 128 * k, idesc, (i % kChunk | k) != 0);
+              umma_commit<kPair>(&s.empty[slot]);
+              if (last) umma_commit<kPair>(&s.acc_full[acc]);
+            }
+            __syncwarp();
+            if (++slot == kRing) { slot = 0; phase ^= 1; }
+            if (last && ++acc == 2) { acc = 0; acc_phase ^= 1; }
+          }
+        }
+      }
+    } else if (warp == 2) {
+      int slot = 0;            // of the next tile's first block
+      uint32_t phases = 0;     // one bit per tail barrier
+      const int b_boxes = (half + kBoxFeatures - 1) / kBoxFeatures;
+      for (int t = group; t < total_tiles && !failed; t += groups) {
+        const WgradTile at = wgrad_tile<kPair>(s.table, g, t);
+        const int rows = at.load % kBR;
+        if (rows != 0) {
+          const int last = (slot + at.blocks - 1) % kRing;
+          if (!mbar_wait(&s.tail[last], (phases >> last) & 1)) { failed = true; break; }
+          phases ^= 1u << last;
+          const int until = (rows + kMmaK - 1) / kMmaK * kMmaK;
+          const int pieces = (until - rows) * 8;  // of 16 bytes, in one box
+          for (int b = 0; b < kABoxes + b_boxes; b++) {
+            unsigned char* const box = (b < kABoxes ? s.a[last] + b * kBoxBytes
+                                                    : s.b[last] + (b - kABoxes) * kBoxBytes) +
+                                       rows * kBoxFeatures * 2;
+            for (int i = lane; i < pieces; i += 32)
+              *reinterpret_cast<uint4*>(box + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) {
+            if (rank == 0) mbar_arrive(&s.full[last]);
+            else mbar_arrive_cluster(map_to_cta(&s.full[last], 0));
+          }
+        }
+        slot = (slot + at.blocks) % kRing;
       }
     }
-  } else if (warp == 2) {
-    int slot = 0;            // of the next tile's first block
-    uint32_t phases = 0;     // one bit per tail barrier
-    const int b_boxes = (half + kBoxFeatures - 1) / kBoxFeatures;
-    for (int t = group; t < total_tiles && !failed; t += groups) {
-      const WgradTile at = wgrad_tile<kPair>(s.table, g, t);
-      const int rows = at.load % kBR;
-      if (rows != 0) {
-        const int last = (slot + at.blocks - 1) % kRing;
-        if (!mbar_wait(&s.tail[last], (phases >> last) & 1)) { failed = true; break; }
-        phases ^= 1u << last;
-        const int until = (rows + kMmaK - 1) / kMmaK * kMmaK;
-        const int pieces = (until - rows) * 8;  // of 16 bytes, in one box
-        for (int b = 0; b < kABoxes + b_boxes; b++) {
-          unsigned char* const box = (b < kABoxes ? s.a[last] + b * kBoxBytes
-                                                  : s.b[last] + (b - kABoxes) * kBoxBytes) +
-                                     rows * kBoxFeatures * 2;
-          for (int i = lane; i < pieces; i += 32)
-            *reinterpret_cast<uint4*>(box + i * 16) = make_uint4(0u, 0u, 0u, 0u);
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) {
-          if (rank == 0) mbar_arrive(&s.full[last]);
-          else mbar_arrive_cluster(map_to_cta(&s.full[last], 0));
-        }
-      }
-      slot = (slot + at.blocks) % kRing;
-    }
-  } else if (warp >= kFirstEpilogueWarp) {
-    const int quarter = warp & 3;
-    unsigned char* const turn = s.turn[quarter];
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegisters));
+    const int quarter = warp & 3;  // the 32 lanes of tensor memory that this warp may read
+    const int cols = g.width / 2;  // of this warp: a multiple of 16
+    const int col0 = (warp - kFirstSumWarp) / 4 * cols;
+    const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)col0;
+    constexpr int kSize = kFloatOut ? 4 : 2;
     int acc = 0;
     uint32_t acc_phase = 0;
-    constexpr int kSize = kFloatOut ? 4 : 2;
-    constexpr int kColumns = 64 / kSize;  // of one turn through shared memory
     for (int t = group; t < total_tiles && !failed; t += groups) {
       const WgradTile at = wgrad_tile<kPair>(s.table, g, t);
-      const int n0 = at.n0 + (int)rank * kBM + quarter * 32;
-      const int columns = min(g.width, g.K - at.k0);
-      unsigned char* const out = static_cast<unsigned char*>(g.out) +
-          (((long long)at.expert * g.N + n0) * g.K + at.k0) * kSize + (lane & 3) * 16;
-      const bool some = at.blocks != 0;
-      if (some) {
+      float sum[kBN / 2];
+#pragma unroll
+      for (int i = 0; i < kBN / 2; i++) sum[i] = 0.f;
+#pragma unroll 1
+      for (int i = 0; i < at.blocks; i += kChunk) {
         if (!mbar_wait(&s.acc_full[acc], acc_phase)) { failed = true; break; }
         tcgen05_after_sync();
-      }
-#pragma unroll 1
-      for (int c0 = 0; c0 < columns; c0 += 32) {
-        uint32_t v[32];
-        if (some) {
-          tmem_load_32(tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(acc * kBN + c0), v);
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+          if (c * 32 >= cols) continue;
+          uint32_t v[32];
+          tmem_load_32(from + (uint32_t)(acc * kBN + c * 32), v);
           tmem_load_wait();
-        } else {
-#pragma unroll
-          for (int i = 0; i < 32; i++) v[i] = 0u;
+          add_columns(sum + c * 32, v);
         }
-#pragma unroll
-        for (int h = 0; h < 32 / kColumns; h++) {
-          uint4 piece[4];
-          if constexpr (kFloatOut) {
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-              piece[i] = make_uint4(v[16 * h + 4 * i], v[16 * h + 4 * i + 1], v[16 * h + 4 * i + 2],
-                                    v[16 * h + 4 * i + 3]);
-          } else {
-            uint32_t w[16];
-#pragma unroll
-            for (int i = 0; i < 16; i++) {
-              const __nv_bfloat162 p = __floats2bfloat162_rn(__uint_as_float(v[2 * i]),
-                                                             __uint_as_float(v[2 * i + 1]));
-              memcpy(&w[i], &p, 4);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-              piece[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-          }
-          __syncwarp();  // everybody has read the last turn
-#pragma unroll
-          for (int i = 0; i < 4; i++)
-            *reinterpret_cast<uint4*>(turn + lane * 64 + ((i ^ (lane >> 1)) & 3) * 16) = piece[i];
-          __syncwarp();
-#pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const int r = i * 8 + (lane >> 2);
-            const int c = c0 + h * kColumns + (lane & 3) * (16 / kSize);
-            if (n0 + r < g.N && c < columns)
-              *reinterpret_cast<uint4*>(out + ((long long)r * g.K + c0 + h * kColumns) * kSize) =
-                  turned_piece(turn, r, lane);
-          }
-        }
-      }
-      if (some) {
         tcgen05_before_sync();
         __syncwarp();
         if (lane == 0) {
           if (rank == 0) mbar_arrive(&s.acc_empty[acc]);
-          else mbar_arrive_cluster(map_to_cta(&s.acc_empty[acc], 0));
+          else mbar_arrive_cluster_relaxed(map_to_cta(&s.acc_empty[acc], 0));
         }
         if (++acc == 2) { acc = 0; acc_phase ^= 1; }
+      }
+      if (failed) break;
+      const int n = at.n0 + (int)rank * kBM + quarter * 32 + lane;
+      const int columns = n < g.N ? min(cols, g.K - at.k0 - col0) : 0;
+      unsigned char* const out = static_cast<unsigned char*>(g.out) +
+          (((long long)at.expert * g.N + n) * g.K + at.k0 + col0) * kSize;
+#pragma unroll
+      for (int c = 0; c < kBN / 2; c += 32 / kSize) {
+        uint32_t w[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          if constexpr (kFloatOut) {
+            w[e] = __float_as_uint(sum[c + e]);
+          } else {
+            const __nv_bfloat162 p = __floats2bfloat162_rn(sum[c + 2 * e], sum[c + 2 * e + 1]);
+            memcpy(&w[e], &p, 4);
+          }
+        }
+        if (c < columns) store_sector(out + c * kSize, w);
       }
     }
   }
@@ -400,7 +409,7 @@ BRT_API int brt_grouped_expert_weight_grad(const void* grads, const void* rows, 
                      "the weight gradient needs in_features %% 16 == 0 and out_features %% 16 == 0 "
                      "(got %lld, %lld)",
                      (long long)in_features, (long long)out_features);
-  BRT_REQUIRE(out != nullptr && aligned_to(out, 16), "out must be 16-byte aligned");
+  BRT_REQUIRE(out != nullptr && aligned_to(out, 32), "out must be 32-byte aligned");
   BRT_REQUIRE(in_features < (1LL << 31) - 512 && out_features < (1LL << 31) - 512,
               "too many features");
   BRT_REQUIRE(total_rows < (1LL << 31) - 1024, "too many rows");
