@@ -14,32 +14,30 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kParts = kCodeBlock * kCodeBlock / 8 / kThreads;  // groups of 8 values per thread
+constexpr int kPitch = kCodeBlock / 4 + 1;                       // words of a turned row
 
 template <int DT, bool kTransposed>
 __global__ void __launch_bounds__(kThreads)
 weight_codes_kernel(const typename Elem<DT>::type* __restrict__ weights,
                     unsigned char* __restrict__ codes, float* __restrict__ scales, int N, int K) {
   __shared__ float s_max[kThreads / 32];
-  __shared__ uint32_t s_turn[kTransposed ? kCodeBlock * (kCodeBlock / 4 + 1) : 1];
+  __shared__ uint32_t s_turn[kTransposed ? kCodeBlock * kPitch : 1];
   const int tid = threadIdx.x;
   const int k0 = blockIdx.x * kCodeBlock, n0 = blockIdx.y * kCodeBlock;
   const long long expert = blockIdx.z;
   const auto* const w = weights + expert * N * (long long)K;
-  const int my_k = (tid & 15) * 8;  // 16 threads hold a row of the block
-  const int my_n = tid >> 4;
-  float v[kParts][8];
-  float amax = 0.f;
+  const int my_k = (tid & 15) * 8;       // 16 threads hold a row of the block,
+  const int my_n = (tid >> 4) * kParts;  // each of them in kParts rows
+  Eight<DT> v[kParts];
 #pragma unroll
   for (int i = 0; i < kParts; i++) {
-    const int n = n0 + my_n + i * (kThreads / 16);
-    if (n < N && k0 + my_k < K) {
-      load_eight<DT>(w + (long long)n * K + k0 + my_k, v[i]);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; e++) v[i][e] = 0.f;
-    }
-    amax = fmaxf(amax, max_abs(v[i]));
+    const int n = n0 + my_n + i;
+    if (n < N && k0 + my_k < K) v[i].load(w + (long long)n * K + k0 + my_k);
+    else v[i].clear();
   }
+  float amax = 0.f;
+#pragma unroll
+  for (int i = 0; i < kParts; i++) amax = fmaxf(amax, v[i].max_abs());
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, d));
   if ((tid & 31) == 0) s_max[tid >> 5] = amax;
@@ -58,30 +56,37 @@ weight_codes_kernel(const typename Elem<DT>::type* __restrict__ weights,
   if constexpr (!kTransposed) {
 #pragma unroll
     for (int i = 0; i < kParts; i++) {
-      const int n = n0 + my_n + i * (kThreads / 16);
+      const int n = n0 + my_n + i;
       if (n < N && k0 + my_k < K)
-        *reinterpret_cast<uint2*>(out + (long long)n * K + k0 + my_k) =
-            encode_eight(v[i], inverse);
+        *reinterpret_cast<uint2*>(out + (long long)n * K + k0 + my_k) = v[i].encode(inverse);
     }
   } else {
-    // row k of s_turn: the codes of 128 neighbouring n, four to a word, one word of padding
-    unsigned char* const turn = reinterpret_cast<unsigned char*>(s_turn);
-    constexpr int kPitch = kCodeBlock + 4;
+    // Row k of s_turn: the codes of 128 neighbouring n, four to a word.  A thread makes words of
+    // four of its rows; their place in a row is exchanged by k / 32, so that the threads of a
+    // warp meet in a bank by twos.
 #pragma unroll
-    for (int i = 0; i < kParts; i++) {
-      const uint2 c = encode_eight(v[i], inverse);
-      const int n = my_n + i * (kThreads / 16);
+    for (int q = 0; q < kParts / 4; q++) {
+      uint2 c[4];
 #pragma unroll
-      for (int e = 0; e < 8; e++)
-        turn[(my_k + e) * kPitch + n] = (unsigned char)((e < 4 ? c.x : c.y) >> (8 * (e & 3)));
+      for (int i = 0; i < 4; i++) c[i] = v[q * 4 + i].encode(inverse);
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const uint32_t pick = (uint32_t)(e & 3) | (uint32_t)(4 + (e & 3)) << 4;
+        const uint32_t lo = __byte_perm(e < 4 ? c[0].x : c[0].y, e < 4 ? c[1].x : c[1].y, pick);
+        const uint32_t hi = __byte_perm(e < 4 ? c[2].x : c[2].y, e < 4 ? c[3].x : c[3].y, pick);
+        const int k = my_k + e;
+        s_turn[k * kPitch + ((my_n / 4 + q) ^ (k >> 5))] = __byte_perm(lo, hi, 0x5410);
+      }
     }
     __syncthreads();
+#pragma unroll
     for (int i = tid; i < kCodeBlock * kCodeBlock / 16; i += kThreads) {
       const int k = i >> 3, n = (i & 7) * 16;
       if (k0 + k < K && n0 + n < N) {
-        const uint32_t* const from = s_turn + k * (kPitch / 4) + n / 4;
+        const uint32_t* const from = s_turn + k * kPitch;
+        const int at = n / 4, x = k >> 5;
         *reinterpret_cast<uint4*>(out + (long long)(k0 + k) * N + n0 + n) =
-            make_uint4(from[0], from[1], from[2], from[3]);
+            make_uint4(from[at ^ x], from[(at + 1) ^ x], from[(at + 2) ^ x], from[(at + 3) ^ x]);
       }
     }
   }

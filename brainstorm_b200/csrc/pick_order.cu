@@ -20,7 +20,7 @@ namespace brt_b200 {
 namespace {
 
 constexpr int kMaxPaths = 1024;
-constexpr int kWarps = 32;
+constexpr int kWarps = 16;
 constexpr int kOneCta = 8192;
 constexpr int kTileMin = 2048;
 
@@ -62,9 +62,11 @@ __device__ __forceinline__ void count_tile(const OrderArgs& a, int* s_hist, int 
   __syncthreads();
 }
 
-// s_hist[warp][bucket] holds the next place of every warp and bucket: hands them out.
+// s_hist[warp][bucket], behind s_base[bucket], is the next place of every warp and bucket: hands
+// them out.
 template <typename P>
-__device__ __forceinline__ void place_tile(const OrderArgs& a, int* s_hist, int lo, int hi) {
+__device__ __forceinline__ void place_tile(const OrderArgs& a, int* s_hist, const int* s_base,
+                                           int lo, int hi) {
   const int buckets = a.paths + 1;
   const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const P* picks = static_cast<const P*>(a.picks);
@@ -76,7 +78,7 @@ __device__ __forceinline__ void place_tile(const OrderArgs& a, int* s_hist, int 
     const int b = i < end ? bucket_of(picks, i, a.paths) : buckets;
     const unsigned same = __match_any_sync(0xffffffffu, b);
     int row = 0;
-    if (b < buckets) row = mine[b] + __popc(same & ((1u << lane) - 1));
+    if (b < buckets) row = s_base[b] + mine[b] + __popc(same & ((1u << lane) - 1));
     __syncwarp();
     if (b < buckets && lane == __ffs(same) - 1) mine[b] += __popc(same);
     __syncwarp();
@@ -123,9 +125,7 @@ __global__ void __launch_bounds__(kWarps * 32) pick_order_kernel(const OrderArgs
   __syncthreads();
   if (threadIdx.x < 32) scan_buckets(s_total, s_base, buckets);
   __syncthreads();
-  for (int i = threadIdx.x; i < warps * buckets; i += blockDim.x) s_hist[i] += s_base[i % buckets];
-  __syncthreads();
-  place_tile<P>(a, s_hist, 0, a.n);
+  place_tile<P>(a, s_hist, s_base, 0, a.n);
 }
 
 template <typename P>
@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(kWarps * 32) pick_place_kernel(const OrderArgs
   if (threadIdx.x < 32) scan_buckets(s_total, s_base, buckets);
   __syncthreads();
   for (int b = threadIdx.x; b < buckets; b += blockDim.x) {
-    int next = s_base[b] + s_before[b];
+    int next = s_before[b];
     for (int w = 0; w < warps; w++) {
       const int c = s_hist[w * buckets + b];
       s_hist[w * buckets + b] = next;
@@ -181,7 +181,7 @@ __global__ void __launch_bounds__(kWarps * 32) pick_place_kernel(const OrderArgs
     if (blockIdx.x == 0 && b < a.paths) a.loads[b] = s_total[b];
   }
   __syncthreads();
-  place_tile<P>(a, s_hist, lo, hi);
+  place_tile<P>(a, s_hist, s_base, lo, hi);
 }
 
 int tile_for(int64_t n) {

@@ -15,7 +15,8 @@
 // nowhere is not looked at.
 //
 // All are bound by HBM (a few operations per byte).  sort and unsort give a warp 2 KB of a cell:
-// a cell is read once for its k copies, and written once.  The backward of unsort
+// a cell is read once for its k copies, and written once; with few cells a warp gets one pick or
+// one access per lane.  The backward of unsort
 // gives a warp one route, so that its dot product stays in the warp and is summed in one fixed
 // order; the k warps of a cell read its gradient from L1 or L2.
 #include "block_codes.cuh"
@@ -25,11 +26,12 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kCtaWarps = kThreads / 32;
-constexpr int kItemsPerWarp = 2;
 
-// VB-byte accesses per lane and item: 2 KB (1 KB of 2-byte accesses) per warp
+// VB-byte accesses per lane and item: 2 KB (1 KB of 2-byte accesses) per warp where there are
+// items enough for the GPU, else one access.
 template <int VB>
 constexpr int kUnroll = VB == 16 ? 4 : 16;
+constexpr int kManyItems = 16;  // per SM
 
 struct SortArgs {
   const unsigned char* cells;
@@ -42,89 +44,103 @@ struct SortArgs {
   long long total_rows;
   int pieces;
   int picks;
+  int group;   // picks of an item
+  int groups;  // items of a piece of a cell
 };
 
-template <int VB>
+// The item of this warp: a piece of a cell for some of its picks.
+struct SortItem {
+  long long cell;
+  int piece, first, last;
+};
+__device__ __forceinline__ SortItem sort_item(const SortArgs& a, long long item) {
+  SortItem it;
+  const long long at = item / a.groups;
+  const int part = (int)(item - at * a.groups);
+  it.cell = at / a.pieces;
+  it.piece = (int)(at - it.cell * a.pieces);
+  it.first = part * a.group;
+  it.last = min(a.picks, it.first + a.group);
+  return it;
+}
+
+template <int VB, int U>
 __global__ void __launch_bounds__(kThreads) sort_cells_kernel(const SortArgs a) {
   using V = typename Chunk<VB>::type;
-  constexpr int U = kUnroll<VB>;
-  constexpr int kPiece = 32 * VB * U;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long first = (long long)blockIdx.x * (kCtaWarps * kItemsPerWarp) + warp;
-#pragma unroll 1
-  for (int i = 0; i < kItemsPerWarp; i++) {
-    const long long item = first + (long long)i * kCtaWarps;
-    if (item >= a.items) return;
-    const long long cell = item / a.pieces;
-    const long long at = (item - cell * a.pieces) * kPiece + lane * VB;
-    const unsigned char* const src = a.cells + cell * a.row_bytes + at;
-    V v[U];
+  const int lane = threadIdx.x & 31;
+  const long long item = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  if (item >= a.items) return;
+  const SortItem it = sort_item(a, item);
+  const long long at = (long long)it.piece * (32 * VB * U) + lane * VB;
+  const unsigned char* const src = a.cells + it.cell * a.row_bytes + at;
+  V v[U];
+#pragma unroll
+  for (int u = 0; u < U; u++)
+    v[u] = at + u * (32 * VB) < a.row_bytes
+               ? load_stream(reinterpret_cast<const V*>(src + u * (32 * VB)))
+               : zero_chunk<V>();
+  const int* const places = a.places + it.cell * a.picks;
+  for (int j = it.first; j < it.last; j++) {
+    const int p = __ldg(places + j);
+    const long long row = p >= 0 ? p : -2LL - p;
+    if (row < 0 || row >= a.total_rows) continue;
+    unsigned char* const dst = a.rows + row * a.row_bytes + at;
 #pragma unroll
     for (int u = 0; u < U; u++)
-      v[u] = at + u * (32 * VB) < a.row_bytes
-                 ? load_stream(reinterpret_cast<const V*>(src + u * (32 * VB)))
-                 : zero_chunk<V>();
-    const int* const places = a.places + cell * a.picks;
-    for (int j = 0; j < a.picks; j++) {
-      const int p = __ldg(places + j);
-      const long long row = p >= 0 ? p : -2LL - p;
-      if (row < 0 || row >= a.total_rows) continue;
-      unsigned char* const dst = a.rows + row * a.row_bytes + at;
-#pragma unroll
-      for (int u = 0; u < U; u++)
-        if (at + u * (32 * VB) < a.row_bytes)
-          *reinterpret_cast<V*>(dst + u * (32 * VB)) = p >= 0 ? v[u] : zero_chunk<V>();
-    }
+      if (at + u * (32 * VB) < a.row_bytes)
+        *reinterpret_cast<V*>(dst + u * (32 * VB)) = p >= 0 ? v[u] : zero_chunk<V>();
   }
 }
 
-constexpr int kCodeUnroll = 4;  // 4 x 256 values per warp and item
+constexpr int kCodeUnroll = 4;  // x 256 values per warp and item
 
 // kPlaced = false: one row per cell, in the order they come (a plain quantisation).
-template <int DT, bool kPlaced>
+template <int DT, int U, bool kPlaced>
 __global__ void __launch_bounds__(kThreads) sort_codes_kernel(const SortArgs a) {
   using T = typename Elem<DT>::type;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long first = (long long)blockIdx.x * (kCtaWarps * kItemsPerWarp) + warp;
-#pragma unroll 1
-  for (int i = 0; i < kItemsPerWarp; i++) {
-    const long long item = first + (long long)i * kCtaWarps;
-    if (item >= a.items) return;
-    const long long cell = item / a.pieces;
-    const long long at = (item - cell * a.pieces) * (256 * kCodeUnroll) + lane * 8;
-    const T* const src = reinterpret_cast<const T*>(a.cells) + cell * a.width + at;
-    uint2 code[kCodeUnroll];
-    float scale[kCodeUnroll];
+  const int lane = threadIdx.x & 31;
+  const long long item = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  if (item >= a.items) return;
+  const SortItem it = sort_item(a, item);
+  const long long at = (long long)it.piece * (256 * U) + lane * 8;
+  const T* const src = reinterpret_cast<const T*>(a.cells) + it.cell * a.width + at;
+  Eight<DT> v[U];
 #pragma unroll
-    for (int u = 0; u < kCodeUnroll; u++) {
-      float v[8];
-      if (at + u * 256 < a.width) {
-        load_eight<DT>(src + u * 256, v);
-      } else {
+  for (int u = 0; u < U; u++) {
+    if (at + u * 256 < a.width) v[u].load(src + u * 256);
+    else v[u].clear();
+  }
+  // 16 lanes hold a block.  Its two quotients are taken by one lane in U of them and handed round:
+  // each is a dozen instructions, and taken by all lanes they cost more than the conversion.
+  float mine = kAmaxFloor;
 #pragma unroll
-        for (int e = 0; e < 8; e++) v[e] = 0.f;
-      }
-      float amax = max_abs(v);  // of the block: 16 lanes hold its 128 values
+  for (int u = 0; u < U; u++) {
+    float amax = v[u].max_abs();
 #pragma unroll
-      for (int d = 8; d > 0; d >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, d));
-      amax = fmaxf(amax, kAmaxFloor);
-      scale[u] = __fdiv_rn(amax, kCodeMax);
-      code[u] = encode_eight(v, __fdiv_rn(kCodeMax, amax));
-    }
-    const int copies = kPlaced ? a.picks : 1;
-    for (int j = 0; j < copies; j++) {
-      const int p = kPlaced ? __ldg(a.places + cell * a.picks + j) : 0;
-      const long long row = !kPlaced ? cell : p >= 0 ? p : -2LL - p;
-      if (row < 0 || row >= a.total_rows) continue;
-      unsigned char* const dst = a.rows + row * a.width + at;
+    for (int d = 8; d > 0; d >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, d));
+    if (lane % U == u) mine = fmaxf(amax, kAmaxFloor);
+  }
+  const float my_scale = __fdiv_rn(mine, kCodeMax);
+  const float my_inverse = __fdiv_rn(kCodeMax, mine);
+  uint2 code[U];
+  float scale[U];
 #pragma unroll
-      for (int u = 0; u < kCodeUnroll; u++) {
-        if (at + u * 256 >= a.width) continue;
-        *reinterpret_cast<uint2*>(dst + u * 256) = p >= 0 ? code[u] : make_uint2(0u, 0u);
-        if ((lane & 15) == 0)
-          a.scales[((at + u * 256) / kCodeBlock) * a.total_rows + row] =
-              p >= 0 ? scale[u] : __fdiv_rn(kAmaxFloor, kCodeMax);
-      }
+  for (int u = 0; u < U; u++) {
+    scale[u] = __shfl_sync(0xffffffffu, my_scale, (lane & 16) + u);
+    code[u] = v[u].encode(__shfl_sync(0xffffffffu, my_inverse, (lane & 16) + u));
+  }
+  for (int j = it.first; j < it.last; j++) {
+    const int p = kPlaced ? __ldg(a.places + it.cell * a.picks + j) : 0;
+    const long long row = !kPlaced ? it.cell : p >= 0 ? p : -2LL - p;
+    if (row < 0 || row >= a.total_rows) continue;
+    unsigned char* const dst = a.rows + row * a.width + at;
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      if (at + u * 256 >= a.width) continue;
+      *reinterpret_cast<uint2*>(dst + u * 256) = p >= 0 ? code[u] : make_uint2(0u, 0u);
+      if ((lane & 15) == 0)
+        a.scales[((at + u * 256) / kCodeBlock) * a.total_rows + row] =
+            p >= 0 ? scale[u] : __fdiv_rn(kAmaxFloor, kCodeMax);
     }
   }
 }
@@ -169,42 +185,59 @@ __device__ __forceinline__ float gate_at(const void* gates, long long i) {
   else return Elem<DT>::to_f32(static_cast<const typename Elem<DT>::type*>(gates)[i]);
 }
 
-template <int DT, int VB, int kGates>
+template <int DT, int VB, int U, int kGates>
 __global__ void __launch_bounds__(kThreads) unsort_cells_kernel(const UnsortArgs a) {
   using V = typename Chunk<VB>::type;
   using P = Pack<DT, VB>;
-  constexpr int U = kUnroll<VB>;
-  constexpr int kPiece = 32 * VB * U;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long item = (long long)blockIdx.x * kCtaWarps + warp;
+  const int lane = threadIdx.x & 31;
+  const long long item = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
   if (item >= a.items) return;
   const long long cell = item / a.pieces;
-  const long long at = (item - cell * a.pieces) * kPiece + lane * VB;
-  const int* const places = a.places + cell * a.picks;
+  const long long at = (item - cell * a.pieces) * (32 * VB * U) + lane * VB;
   float sum[U][P::kValues];
 #pragma unroll
   for (int u = 0; u < U; u++)
 #pragma unroll
     for (int e = 0; e < P::kValues; e++) sum[u][e] = 0.f;
-#pragma unroll 2
-  for (int j = 0; j < a.picks; j++) {
-    const int p = __ldg(places + j);
-    if (p < 0 || p >= a.total_rows) continue;
-    const float gate = gate_at<DT, kGates>(a.gates, cell * a.picks + j);
-    const unsigned char* const src = a.rows + (long long)p * a.row_bytes + at;
-    V raw[U];
+  // two rows are on their way at a time (more with short pieces)
+  constexpr int kAtOnce = U * VB >= 64 || VB < 16 ? 2 : 8;
+  for (int j0 = 0; j0 < a.picks; j0 += 32) {
+    // a lane for each pick: its place and gate come with one access each
+    int my_place = -1;
+    float my_gate = 0.f;
+    if (j0 + lane < a.picks) {
+      const long long route = cell * a.picks + j0 + lane;
+      my_place = __ldg(a.places + route);
+      my_gate = gate_at<DT, kGates>(a.gates, route);
+    }
+    const int until = min(32, a.picks - j0);
+    for (int j = 0; j < until; j += kAtOnce) {
+      V raw[kAtOnce][U];
+      int place[kAtOnce];
 #pragma unroll
-    for (int u = 0; u < U; u++)
-      raw[u] = at + u * (32 * VB) < a.row_bytes
-                   ? load_stream(reinterpret_cast<const V*>(src + u * (32 * VB)))
-                   : zero_chunk<V>();
+      for (int h = 0; h < kAtOnce; h++) {
+        place[h] = __shfl_sync(0xffffffffu, my_place, (j + h) & 31);
+        if (j + h >= until || place[h] >= a.total_rows) place[h] = -1;
+        const unsigned char* const src = a.rows + (long long)place[h] * a.row_bytes + at;
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-      float v[P::kValues];
-      P::values(raw[u], v);
+        for (int u = 0; u < U; u++)
+          raw[h][u] = place[h] >= 0 && at + u * (32 * VB) < a.row_bytes
+                          ? load_stream(reinterpret_cast<const V*>(src + u * (32 * VB)))
+                          : zero_chunk<V>();
+      }
 #pragma unroll
-      for (int e = 0; e < P::kValues; e++)
-        sum[u][e] = kGates == 0 ? sum[u][e] + v[e] : fmaf(gate, v[e], sum[u][e]);
+      for (int h = 0; h < kAtOnce; h++) {
+        const float gate = __shfl_sync(0xffffffffu, my_gate, (j + h) & 31);
+        if (place[h] < 0) continue;  // the whole warp: its gate may be anything
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+          float v[P::kValues];
+          P::values(raw[h][u], v);
+#pragma unroll
+          for (int e = 0; e < P::kValues; e++)
+            sum[u][e] = kGates == 0 ? sum[u][e] + v[e] : fmaf(gate, v[e], sum[u][e]);
+        }
+      }
     }
   }
   unsigned char* const dst = a.cells + cell * a.row_bytes + at;
@@ -243,22 +276,33 @@ __global__ void __launch_bounds__(kThreads) unsort_backward_kernel(const BackArg
     const float gate = live ? gate_at<DT, kGates>(a.gates, route) : 0.f;
     const unsigned char* const grad = a.cell_grads + route / a.picks * a.row_bytes;
     const bool dots = live && a.gate_grads != nullptr;
-#pragma unroll 4
-    for (long long at = lane * VB; at < a.row_bytes; at += 32 * VB) {
-      float g[P::kValues], out[P::kValues];
-      if (live) {
-        P::values(__ldg(reinterpret_cast<const V*>(grad + at)), g);
-        if (dots) {
-          float r[P::kValues];
-          P::values(load_stream(reinterpret_cast<const V*>(a.rows + row * a.row_bytes + at)), r);
+    constexpr int U = VB == 16 ? 4 : 8;
+    for (long long at = lane * VB; at < a.row_bytes; at += 32 * VB * U) {
+      V g[U], r[U];
 #pragma unroll
-          for (int e = 0; e < P::kValues; e++) dot = fmaf(g[e], r[e], dot);
-        }
+      for (int u = 0; u < U; u++) {
+        const long long o = at + u * (32 * VB);
+        const bool real = live && o < a.row_bytes;
+        g[u] = real ? __ldg(reinterpret_cast<const V*>(grad + o)) : zero_chunk<V>();
+        r[u] = real && dots
+                   ? load_stream(reinterpret_cast<const V*>(a.rows + row * a.row_bytes + o))
+                   : zero_chunk<V>();
       }
-      if (a.row_grads != nullptr) {
 #pragma unroll
-        for (int e = 0; e < P::kValues; e++) out[e] = live ? gate * g[e] : 0.f;
-        store_stream(reinterpret_cast<V*>(a.row_grads + row * a.row_bytes + at), P::chunk(out));
+      for (int u = 0; u < U; u++) {
+        const long long o = at + u * (32 * VB);
+        float gv[P::kValues], rv[P::kValues];
+        P::values(g[u], gv);
+        P::values(r[u], rv);
+        if (dots && o < a.row_bytes) {
+#pragma unroll
+          for (int e = 0; e < P::kValues; e++) dot = fmaf(gv[e], rv[e], dot);
+        }
+        if (a.row_grads != nullptr && o < a.row_bytes) {
+#pragma unroll
+          for (int e = 0; e < P::kValues; e++) gv[e] = live ? gate * gv[e] : 0.f;
+          store_stream(reinterpret_cast<V*>(a.row_grads + row * a.row_bytes + o), P::chunk(gv));
+        }
       }
     }
   }
@@ -280,33 +324,68 @@ int access_bytes(long long row_bytes, int element, const void* a, const void* b,
       return vb;
   return element;
 }
-template <int VB>
-int pieces_of(long long row_bytes) {
-  return (int)((row_bytes + 32 * VB * kUnroll<VB> - 1) / (32 * VB * kUnroll<VB>));
+// Few items: one warp per CTA spreads them over the SMs.
+struct Shape {
+  unsigned grid = 0, threads = 0;
+  explicit Shape(long long items) {
+    const long long most = (long long)sm_count() * kManyItems;
+    threads = items >= most ? kThreads : items * 4 >= most ? 128 : 32;
+    const long long ctas = (items + threads / 32 - 1) / (threads / 32);
+    grid = ctas <= 0x7fffffffLL ? (unsigned)ctas : 0;
+  }
+};
+template <int VB, int U>
+long long pieces_of(long long row_bytes) {
+  return (row_bytes + 32 * VB * U - 1) / (32 * VB * U);
 }
-int pieces_of(long long row_bytes, int vb) {
-  return vb == 16 ? pieces_of<16>(row_bytes) : vb == 4 ? pieces_of<4>(row_bytes)
-                                                       : pieces_of<2>(row_bytes);
-}
+bool many(long long items) { return items >= (long long)sm_count() * kManyItems; }
 
-template <int DT, int VB>
-int launch_unsort(const UnsortArgs& a, int gates, cudaStream_t st) {
-  const long long grid = (a.items + kCtaWarps - 1) / kCtaWarps;
-  BRT_REQUIRE(grid <= 0x7fffffffLL, "too many cells for one launch");
+template <int DT, int VB, int U>
+int launch_unsort(UnsortArgs a, long long cells, int gates, cudaStream_t st) {
+  a.pieces = (int)pieces_of<VB, U>(a.row_bytes);
+  a.items = cells * a.pieces;
+  const Shape s(a.items);
+  BRT_REQUIRE(s.grid > 0, "too many cells for one launch");
   const KernelTimer timer("unsort_cells_kernel", st);
-  if (gates == 0) unsort_cells_kernel<DT, VB, 0><<<(unsigned)grid, kThreads, 0, st>>>(a);
-  else if (gates == 1) unsort_cells_kernel<DT, VB, 1><<<(unsigned)grid, kThreads, 0, st>>>(a);
-  else unsort_cells_kernel<DT, VB, 2><<<(unsigned)grid, kThreads, 0, st>>>(a);
+  if (gates == 0) unsort_cells_kernel<DT, VB, U, 0><<<s.grid, s.threads, 0, st>>>(a);
+  else if (gates == 1) unsort_cells_kernel<DT, VB, U, 1><<<s.grid, s.threads, 0, st>>>(a);
+  else unsort_cells_kernel<DT, VB, U, 2><<<s.grid, s.threads, 0, st>>>(a);
   note_launch();
   BRT_LAUNCH_CHECK("unsort_cells_kernel");
   return BRT_OK;
 }
+template <int DT, int VB>
+int launch_unsort(const UnsortArgs& a, long long cells, int gates, cudaStream_t st) {
+  if (many(cells * pieces_of<VB, kUnroll<VB>>(a.row_bytes)))
+    return launch_unsort<DT, VB, kUnroll<VB>>(a, cells, gates, st);
+  return launch_unsort<DT, VB, 1>(a, cells, gates, st);
+}
 template <int DT>
-int launch_unsort(const UnsortArgs& a, int vb, int gates, cudaStream_t st) {
-  if (vb == 16) return launch_unsort<DT, 16>(a, gates, st);
+int launch_unsort(const UnsortArgs& a, long long cells, int vb, int gates, cudaStream_t st) {
+  if (vb == 16) return launch_unsort<DT, 16>(a, cells, gates, st);
   if constexpr (DT != BRT_F32)
-    if (vb == 2) return launch_unsort<DT, 2>(a, gates, st);
-  return launch_unsort<DT, 4>(a, gates, st);
+    if (vb == 2) return launch_unsort<DT, 2>(a, cells, gates, st);
+  return launch_unsort<DT, 4>(a, cells, gates, st);
+}
+
+// Items of whole cells read each cell once; where they are too few to fill the GPU an item is
+// one pick of a short piece.
+template <int VB>
+int launch_sort(SortArgs a, long long cells, cudaStream_t st) {
+  constexpr int kLong = kUnroll<VB>;
+  const bool whole = many(cells * pieces_of<VB, kLong>(a.row_bytes));
+  a.pieces = (int)(whole ? pieces_of<VB, kLong>(a.row_bytes) : pieces_of<VB, 1>(a.row_bytes));
+  a.group = whole ? a.picks : 1;
+  a.groups = whole ? 1 : a.picks;
+  a.items = cells * a.pieces * a.groups;
+  const Shape s(a.items);
+  BRT_REQUIRE(s.grid > 0, "too many cells for one launch");
+  const KernelTimer timer("sort_cells_kernel", st);
+  if (whole) sort_cells_kernel<VB, kLong><<<s.grid, s.threads, 0, st>>>(a);
+  else sort_cells_kernel<VB, 1><<<s.grid, s.threads, 0, st>>>(a);
+  note_launch();
+  BRT_LAUNCH_CHECK("sort_cells_kernel");
+  return BRT_OK;
 }
 
 template <int DT, int VB>
@@ -328,21 +407,28 @@ int launch_back(const BackArgs& a, int vb, int gates, cudaStream_t st) {
   return launch_back<DT, 4>(a, gates, st);
 }
 
-template <bool kPlaced>
-int launch_codes(SortArgs a, long long cells, int dtype, cudaStream_t st) {
-  a.pieces = (int)((a.width + 256 * kCodeUnroll - 1) / (256 * kCodeUnroll));
-  a.items = cells * a.pieces;
-  const long long per = kCtaWarps * kItemsPerWarp;
-  const long long grid = (a.items + per - 1) / per;
-  BRT_REQUIRE(grid <= 0x7fffffffLL, "too many rows for one launch");
+template <int DT, bool kPlaced>
+int launch_codes(SortArgs a, long long cells, cudaStream_t st) {
+  constexpr long long kLong = 256 * kCodeUnroll;
+  const bool whole = many(cells * ((a.width + kLong - 1) / kLong));
+  a.pieces = (int)(whole ? (a.width + kLong - 1) / kLong : (a.width + 255) / 256);
+  a.group = whole ? a.picks : 1;
+  a.groups = whole ? 1 : a.picks;
+  a.items = cells * a.pieces * a.groups;
+  const Shape s(a.items);
+  BRT_REQUIRE(s.grid > 0, "too many rows for one launch");
   const KernelTimer timer("sort_codes_kernel", st);
-  const unsigned g = (unsigned)grid;
-  if (dtype == BRT_F32) sort_codes_kernel<BRT_F32, kPlaced><<<g, kThreads, 0, st>>>(a);
-  else if (dtype == BRT_F16) sort_codes_kernel<BRT_F16, kPlaced><<<g, kThreads, 0, st>>>(a);
-  else sort_codes_kernel<BRT_BF16, kPlaced><<<g, kThreads, 0, st>>>(a);
+  if (whole) sort_codes_kernel<DT, kCodeUnroll, kPlaced><<<s.grid, s.threads, 0, st>>>(a);
+  else sort_codes_kernel<DT, 1, kPlaced><<<s.grid, s.threads, 0, st>>>(a);
   note_launch();
   BRT_LAUNCH_CHECK("sort_codes_kernel");
   return BRT_OK;
+}
+template <bool kPlaced>
+int launch_codes(const SortArgs& a, long long cells, int dtype, cudaStream_t st) {
+  if (dtype == BRT_F32) return launch_codes<BRT_F32, kPlaced>(a, cells, st);
+  if (dtype == BRT_F16) return launch_codes<BRT_F16, kPlaced>(a, cells, st);
+  return launch_codes<BRT_BF16, kPlaced>(a, cells, st);
 }
 
 bool known_dtype(int dtype) { return dtype == BRT_F32 || dtype == BRT_F16 || dtype == BRT_BF16; }
@@ -379,18 +465,9 @@ BRT_API int brt_sort_cells(const void* cells, const int32_t* places, void* rows,
   a.total_rows = cell_num * pick_num;
   a.picks = pick_num;
   const int vb = access_bytes(a.row_bytes, dtype_size(dtype), cells, rows, nullptr);
-  a.pieces = pieces_of(a.row_bytes, vb);
-  a.items = cell_num * a.pieces;
-  const long long per = kCtaWarps * kItemsPerWarp;
-  const long long grid = (a.items + per - 1) / per;
-  BRT_REQUIRE(grid <= 0x7fffffffLL, "too many cells for one launch");
-  const KernelTimer timer("sort_cells_kernel", st);
-  if (vb == 16) sort_cells_kernel<16><<<(unsigned)grid, kThreads, 0, st>>>(a);
-  else if (vb == 4) sort_cells_kernel<4><<<(unsigned)grid, kThreads, 0, st>>>(a);
-  else sort_cells_kernel<2><<<(unsigned)grid, kThreads, 0, st>>>(a);
-  note_launch();
-  BRT_LAUNCH_CHECK("sort_cells_kernel");
-  return BRT_OK;
+  if (vb == 16) return launch_sort<16>(a, cell_num, st);
+  if (vb == 4) return launch_sort<4>(a, cell_num, st);
+  return launch_sort<2>(a, cell_num, st);
 }
 
 BRT_API int brt_sort_cells_fp8(const void* cells, const int32_t* places, void* codes,
@@ -455,13 +532,11 @@ BRT_API int brt_unsort_cells(const void* rows, const int32_t* places, const void
   a.total_rows = cell_num * pick_num;
   a.picks = pick_num;
   const int vb = access_bytes(a.row_bytes, dtype_size(dtype), cells, rows, nullptr);
-  a.pieces = pieces_of(a.row_bytes, vb);
-  a.items = cell_num * a.pieces;
   const int kind = gates == nullptr ? 0 : gates_dtype == BRT_F32 ? 1 : 2;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dtype == BRT_F32) return launch_unsort<BRT_F32>(a, vb, kind, st);
-  if (dtype == BRT_F16) return launch_unsort<BRT_F16>(a, vb, kind, st);
-  return launch_unsort<BRT_BF16>(a, vb, kind, st);
+  if (dtype == BRT_F32) return launch_unsort<BRT_F32>(a, cell_num, vb, kind, st);
+  if (dtype == BRT_F16) return launch_unsort<BRT_F16>(a, cell_num, vb, kind, st);
+  return launch_unsort<BRT_BF16>(a, cell_num, vb, kind, st);
 }
 
 BRT_API int brt_unsort_cells_backward(const void* cell_grads, const void* rows,
