@@ -20,7 +20,9 @@ namespace brt_b200 {
 namespace {
 
 constexpr int kMaxPaths = 1024;
-constexpr int kWarps = 16;
+constexpr int kWarps = 32;       // of a tile's CTA
+constexpr int kOneCtaWarps = 16;  // fewer histograms to add up
+constexpr int kBatch = 4;         // steps of 32 picks fetched together
 constexpr int kOneCta = 8192;
 constexpr int kTileMin = 2048;
 
@@ -52,12 +54,19 @@ __device__ __forceinline__ void count_tile(const OrderArgs& a, int* s_hist, int 
   const int run = a.tile / warps;
   const int end = min(lo + (warp + 1) * run, hi);
   int* const mine = s_hist + warp * buckets;
-  for (int i0 = lo + warp * run; i0 < end; i0 += 32) {
-    const int i = i0 + lane;
-    const int b = i < end ? bucket_of(picks, i, a.paths) : buckets;
-    const unsigned same = __match_any_sync(0xffffffffu, b);
-    if (b < buckets && lane == __ffs(same) - 1) mine[b] += __popc(same);
-    __syncwarp();
+  for (int i0 = lo + warp * run; i0 < end; i0 += 32 * kBatch) {
+    int b[kBatch];
+#pragma unroll
+    for (int s = 0; s < kBatch; s++) {
+      const int i = i0 + s * 32 + lane;
+      b[s] = i < end ? bucket_of(picks, i, a.paths) : buckets;
+    }
+#pragma unroll
+    for (int s = 0; s < kBatch; s++) {
+      const unsigned same = __match_any_sync(0xffffffffu, b[s]);
+      if (b[s] < buckets && lane == __ffs(same) - 1) mine[b[s]] += __popc(same);
+      __syncwarp();
+    }
   }
   __syncthreads();
 }
@@ -73,34 +82,44 @@ __device__ __forceinline__ void place_tile(const OrderArgs& a, int* s_hist, cons
   const int run = a.tile / warps;
   const int end = min(lo + (warp + 1) * run, hi);
   int* const mine = s_hist + warp * buckets;
-  for (int i0 = lo + warp * run; i0 < end; i0 += 32) {
-    const int i = i0 + lane;
-    const int b = i < end ? bucket_of(picks, i, a.paths) : buckets;
-    const unsigned same = __match_any_sync(0xffffffffu, b);
-    int row = 0;
-    if (b < buckets) row = s_base[b] + mine[b] + __popc(same & ((1u << lane) - 1));
-    __syncwarp();
-    if (b < buckets && lane == __ffs(same) - 1) mine[b] += __popc(same);
-    __syncwarp();
-    if (b < buckets) a.places[i] = b < a.paths ? row : -2 - row;
+  for (int i0 = lo + warp * run; i0 < end; i0 += 32 * kBatch) {
+    int b[kBatch];
+#pragma unroll
+    for (int s = 0; s < kBatch; s++) {
+      const int i = i0 + s * 32 + lane;
+      b[s] = i < end ? bucket_of(picks, i, a.paths) : buckets;
+    }
+#pragma unroll
+    for (int s = 0; s < kBatch; s++) {
+      const unsigned same = __match_any_sync(0xffffffffu, b[s]);
+      int row = 0;
+      if (b[s] < buckets) row = s_base[b[s]] + mine[b[s]] + __popc(same & ((1u << lane) - 1));
+      __syncwarp();
+      if (b[s] < buckets && lane == __ffs(same) - 1) mine[b[s]] += __popc(same);
+      __syncwarp();
+      if (b[s] < buckets) a.places[i0 + s * 32 + lane] = b[s] < a.paths ? row : -2 - row;
+    }
   }
 }
 
-// s_base[bucket] <- exclusive sums of s_total over the buckets (one warp).
+// s_base[bucket] <- exclusive sums of s_total over the buckets (one warp, each lane a run of
+// neighbouring buckets).
 __device__ __forceinline__ void scan_buckets(const int* s_total, int* s_base, int buckets) {
   const int lane = threadIdx.x & 31;
-  int before = 0;
-  for (int b0 = 0; b0 < buckets; b0 += 32) {
-    const int b = b0 + lane;
-    const int mine = b < buckets ? s_total[b] : 0;
-    int incl = mine;
+  const int per = (buckets + 31) / 32;
+  const int first = lane * per, last = min(first + per, buckets);
+  int mine = 0;
+  for (int b = first; b < last; b++) mine += s_total[b];
+  int incl = mine;
 #pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int up = __shfl_up_sync(0xffffffffu, incl, d);
-      if (lane >= d) incl += up;
-    }
-    if (b < buckets) s_base[b] = before + incl - mine;
-    before += __shfl_sync(0xffffffffu, incl, 31);
+  for (int d = 1; d < 32; d <<= 1) {
+    const int up = __shfl_up_sync(0xffffffffu, incl, d);
+    if (lane >= d) incl += up;
+  }
+  int next = incl - mine;
+  for (int b = first; b < last; b++) {
+    s_base[b] = next;
+    next += s_total[b];
   }
 }
 
@@ -114,6 +133,7 @@ __global__ void __launch_bounds__(kWarps * 32) pick_order_kernel(const OrderArgs
   count_tile<P>(a, s_hist, 0, a.n);
   for (int b = threadIdx.x; b < buckets; b += blockDim.x) {
     int sum = 0;
+#pragma unroll 8
     for (int w = 0; w < warps; w++) {
       const int c = s_hist[w * buckets + b];
       s_hist[w * buckets + b] = sum;
@@ -159,7 +179,7 @@ __global__ void __launch_bounds__(kWarps * 32) pick_place_kernel(const OrderArgs
   for (int at = threadIdx.x; at < groups * buckets; at += blockDim.x) {
     const int b = at % buckets;
     int total = 0, before = 0;
-#pragma unroll 4
+#pragma unroll 8
     for (int t = at / buckets; t < a.tiles; t += groups) {
       const int c = a.counts[t * buckets + b];
       total += c;
@@ -210,7 +230,7 @@ int launch_order(OrderArgs a, cudaStream_t st) {
   const KernelTimer timer("pick_order", st);
   if (a.n <= kOneCta) {
     int warps = (a.n + 31) / 32;
-    if (warps > kWarps) warps = kWarps;
+    if (warps > kOneCtaWarps) warps = kOneCtaWarps;
     a.tile = (int)round_up((size_t)a.n, (size_t)warps * 32);
     const size_t smem = (size_t)(warps + 2) * buckets * sizeof(int);
     pick_order_kernel<P><<<1, warps * 32, smem, st>>>(a);

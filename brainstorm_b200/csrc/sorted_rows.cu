@@ -32,6 +32,7 @@ constexpr int kCtaWarps = kThreads / 32;
 template <int VB>
 constexpr int kUnroll = VB == 16 ? 4 : 16;
 constexpr int kManyItems = 16;  // per SM
+constexpr int kManyCells = 4;   // per SM, where long items also save reads
 
 struct SortArgs {
   const unsigned char* cells;
@@ -118,7 +119,7 @@ __global__ void __launch_bounds__(kThreads) sort_codes_kernel(const SortArgs a) 
     float amax = v[u].max_abs();
 #pragma unroll
     for (int d = 8; d > 0; d >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, d));
-    if (lane % U == u) mine = fmaxf(amax, kAmaxFloor);
+    if ((lane & 15) % U == u) mine = fmaxf(amax, kAmaxFloor);
   }
   const float my_scale = __fdiv_rn(mine, kCodeMax);
   const float my_inverse = __fdiv_rn(kCodeMax, mine);
@@ -199,8 +200,8 @@ __global__ void __launch_bounds__(kThreads) unsort_cells_kernel(const UnsortArgs
   for (int u = 0; u < U; u++)
 #pragma unroll
     for (int e = 0; e < P::kValues; e++) sum[u][e] = 0.f;
-  // two rows are on their way at a time (more with short pieces)
-  constexpr int kAtOnce = U * VB >= 64 || VB < 16 ? 2 : 8;
+  // rows on their way at a time: as many as registers allow without losing warps
+  constexpr int kAtOnce = VB < 16 && U > 1 ? 1 : U > 1 ? 2 : 8;
   for (int j0 = 0; j0 < a.picks; j0 += 32) {
     // a lane for each pick: its place and gate come with one access each
     int my_place = -1;
@@ -338,7 +339,13 @@ template <int VB, int U>
 long long pieces_of(long long row_bytes) {
   return (row_bytes + 32 * VB * U - 1) / (32 * VB * U);
 }
-bool many(long long items) { return items >= (long long)sm_count() * kManyItems; }
+bool many(long long items, int per_sm) { return items >= (long long)sm_count() * per_sm; }
+// Accesses per lane and item: 3 where that leaves fewer lanes without work at a row's end.
+template <int VB>
+bool by_threes(long long row_bytes) {
+  const long long accesses = (row_bytes + 32 * VB - 1) / (32 * VB);
+  return VB == 16 && (accesses + 2) / 3 * 3 < (accesses + 3) / 4 * 4;
+}
 
 template <int DT, int VB, int U>
 int launch_unsort(UnsortArgs a, long long cells, int gates, cudaStream_t st) {
@@ -356,8 +363,11 @@ int launch_unsort(UnsortArgs a, long long cells, int gates, cudaStream_t st) {
 }
 template <int DT, int VB>
 int launch_unsort(const UnsortArgs& a, long long cells, int gates, cudaStream_t st) {
-  if (many(cells * pieces_of<VB, kUnroll<VB>>(a.row_bytes)))
+  if (many(cells * pieces_of<VB, kUnroll<VB>>(a.row_bytes), kManyItems)) {
+    if (by_threes<VB>(a.row_bytes))
+      return launch_unsort<DT, VB, VB == 16 ? 3 : 1>(a, cells, gates, st);
     return launch_unsort<DT, VB, kUnroll<VB>>(a, cells, gates, st);
+  }
   return launch_unsort<DT, VB, 1>(a, cells, gates, st);
 }
 template <int DT>
@@ -373,7 +383,7 @@ int launch_unsort(const UnsortArgs& a, long long cells, int vb, int gates, cudaS
 template <int VB>
 int launch_sort(SortArgs a, long long cells, cudaStream_t st) {
   constexpr int kLong = kUnroll<VB>;
-  const bool whole = many(cells * pieces_of<VB, kLong>(a.row_bytes));
+  const bool whole = many(cells * pieces_of<VB, kLong>(a.row_bytes), kManyCells);
   a.pieces = (int)(whole ? pieces_of<VB, kLong>(a.row_bytes) : pieces_of<VB, 1>(a.row_bytes));
   a.group = whole ? a.picks : 1;
   a.groups = whole ? 1 : a.picks;
@@ -409,16 +419,18 @@ int launch_back(const BackArgs& a, int vb, int gates, cudaStream_t st) {
 
 template <int DT, bool kPlaced>
 int launch_codes(SortArgs a, long long cells, cudaStream_t st) {
-  constexpr long long kLong = 256 * kCodeUnroll;
-  const bool whole = many(cells * ((a.width + kLong - 1) / kLong));
-  a.pieces = (int)(whole ? (a.width + kLong - 1) / kLong : (a.width + 255) / 256);
+  const bool threes = by_threes<16>(a.width * 2);  // 256 values per access, whatever their type
+  const long long length = 256 * (threes ? 3 : kCodeUnroll);
+  const bool whole = many(cells * ((a.width + length - 1) / length), kManyCells);
+  a.pieces = (int)(whole ? (a.width + length - 1) / length : (a.width + 255) / 256);
   a.group = whole ? a.picks : 1;
   a.groups = whole ? 1 : a.picks;
   a.items = cells * a.pieces * a.groups;
   const Shape s(a.items);
   BRT_REQUIRE(s.grid > 0, "too many rows for one launch");
   const KernelTimer timer("sort_codes_kernel", st);
-  if (whole) sort_codes_kernel<DT, kCodeUnroll, kPlaced><<<s.grid, s.threads, 0, st>>>(a);
+  if (whole && threes) sort_codes_kernel<DT, 3, kPlaced><<<s.grid, s.threads, 0, st>>>(a);
+  else if (whole) sort_codes_kernel<DT, kCodeUnroll, kPlaced><<<s.grid, s.threads, 0, st>>>(a);
   else sort_codes_kernel<DT, 1, kPlaced><<<s.grid, s.threads, 0, st>>>(a);
   note_launch();
   BRT_LAUNCH_CHECK("sort_codes_kernel");
