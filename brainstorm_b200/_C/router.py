@@ -734,6 +734,9 @@ def order_picks(picks: torch.Tensor, path_num: int):
     go nowhere; their places are ``-2 - row``, naming the row at the end of the buffer that stays
     empty.  A place may be set to -1 afterwards to leave out a pick altogether.  At most 1024
     paths; nothing is read back to the host."""
+    done = _lib.host_ops().order_picks(picks, path_num)
+    if done is not None:
+        return done
     _check_cuda(picks, "picks")
     if picks.dim() != 2 or picks.size(1) < 1:
         raise RuntimeError(f"picks must be [cells, k], got {tuple(picks.shape)}")
@@ -860,6 +863,9 @@ def sort_cells(in_data: torch.Tensor, places: torch.Tensor) -> torch.Tensor:
     """``rows[places[t, j]] = in_data[t]``: cells [cells, ...] to [cells * k, ...] rows sorted by
     path, ``places`` as ``order_picks`` returned them.  Rows that stay empty are zeros.  The
     gradient of a cell is the sum of its rows' gradients (fp32, rounded once)."""
+    done = _lib.host_ops().sort_cells(in_data, places)
+    if done is not None:
+        return done
     places = _check_places(places, in_data, "in_data")
     if in_data.size(0) != places.size(0):
         raise RuntimeError(f"{in_data.size(0)} cells but places of {places.size(0)}")
@@ -872,6 +878,9 @@ def sort_cells_fp8(in_data: torch.Tensor, places: torch.Tensor):
     """``sort_cells`` followed by ``quantize_rows`` of ``_C.expert`` in one pass over the cells:
     (codes [cells * k, width] float8_e4m3fn, scales [cells * k, ceil(width / 128)] fp32).  The
     width must be a multiple of 16.  No gradient: train through ``sort_cells``."""
+    done = _lib.host_ops().sort_cells_fp8(in_data, places)
+    if done is not None:
+        return done
     places = _check_places(places, in_data, "in_data")
     if in_data.dim() != 2 or in_data.size(0) != places.size(0):
         raise RuntimeError(f"in_data must be [{places.size(0)}, width], got "
@@ -898,6 +907,9 @@ def unsort_cells(rows: torch.Tensor, places: torch.Tensor,
     for a cell whose picks all go nowhere.  ``gates`` [cells, k] fp32 or of the rows' type (their
     values at picks that go nowhere do not matter), or None for the plain sum.  fp32 sums in the
     order of j, rounded once.  Differentiable in rows and gates; empty rows get zero gradients."""
+    done = _lib.host_ops().unsort_cells(rows, places, gates)
+    if done is not None:
+        return done
     places = _check_places(places, rows, "rows")
     if rows.size(0) != places.numel():
         raise RuntimeError(f"{rows.size(0)} rows but {places.numel()} places")

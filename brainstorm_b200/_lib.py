@@ -163,6 +163,7 @@ class _DeclinesAll:
         return None
 
     route_scores = dispatch = combine = scan
+    order_picks = sort_cells = sort_cells_fp8 = unsort_cells = scan
 
 
 def host_ops():

@@ -15,9 +15,13 @@
 #include <ATen/cuda/EmptyTensor.h>
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAFunctions.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/version.h>
 
@@ -406,6 +410,225 @@ PyObject* combine(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// ---- compact picks: rows sorted by path, back to cells, and their gradients -----------------
+
+bool is_places(const at::Tensor* t) { return int32c(t, 2) && t->numel() > 0; }
+bool wants_grad(const at::Tensor* t) {
+  return t != nullptr && t->requires_grad() && c10::GradMode::is_enabled();
+}
+void done(int rc) { TORCH_CHECK(rc == BRT_OK, brt_last_error()); }
+void* stream_of(const at::Tensor& t) {
+  return c10::cuda::getCurrentCUDAStream(t.get_device()).stream();
+}
+at::Tensor like_rows(const at::Tensor& t, int64_t rows) {
+  c10::SmallVector<int64_t, 6> shape(t.sizes().begin(), t.sizes().end());
+  shape[0] = rows;
+  return empty(shape, t.scalar_type(), t.device());
+}
+
+// The kernels over contiguous tensors; `cells` and `rows` not empty.
+at::Tensor sorted_rows(const at::Tensor& cells, const at::Tensor& places) {
+  const int64_t T = places.size(0), k = places.size(1);
+  at::Tensor rows = like_rows(cells, T * k);
+  done(brt_sort_cells(cells.data_ptr(), static_cast<const int32_t*>(places.data_ptr()),
+                      rows.data_ptr(), T, (int)k, cells.numel() / T, dtype_of(cells),
+                      stream_of(cells)));
+  return rows;
+}
+at::Tensor cells_of(const at::Tensor& rows, const at::Tensor& places, const at::Tensor& gates) {
+  const int64_t T = places.size(0), k = places.size(1);
+  at::Tensor cells = like_rows(rows, T);
+  done(brt_unsort_cells(rows.data_ptr(), static_cast<const int32_t*>(places.data_ptr()),
+                        data_or_null(gates), cells.data_ptr(), T, (int)k,
+                        rows.numel() / (T * k), dtype_of(rows),
+                        gates.defined() ? dtype_of(gates) : 0, stream_of(rows)));
+  return cells;
+}
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// The gradients are not differentiable themselves: asking for that says so.
+variable_list once(variable_list grads) {
+  if (!c10::GradMode::is_enabled()) return grads;
+  const auto error = std::make_shared<torch::autograd::DelayedError>(
+      "the gradients of sorted rows cannot be differentiated", (int64_t)grads.size());
+  for (at::Tensor& g : grads)
+    if (g.defined()) g = g.detach().requires_grad_();
+  return (*error)(std::move(grads));
+}
+
+struct SortCells : public torch::autograd::Function<SortCells> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& cells,
+                            const at::Tensor& places) {
+    ctx->save_for_backward({places});
+    return sorted_rows(cells, places);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    const c10::cuda::CUDAGuard guard(saved[0].device());
+    return once({cells_of(grads[0].contiguous(), saved[0], {}), at::Tensor()});
+  }
+};
+
+struct SumCells : public torch::autograd::Function<SumCells> {  // unsort without gates
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& rows,
+                            const at::Tensor& places) {
+    ctx->save_for_backward({places});
+    return cells_of(rows, places, {});
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    const c10::cuda::CUDAGuard guard(saved[0].device());
+    return once({sorted_rows(grads[0].contiguous(), saved[0]), at::Tensor()});
+  }
+};
+
+struct UnsortCells : public torch::autograd::Function<UnsortCells> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& rows,
+                            const at::Tensor& places, const at::Tensor& gates) {
+    // the rows are only read again for the gradient of the gates
+    ctx->save_for_backward({gates.requires_grad() ? rows : at::Tensor(), places, gates});
+    return cells_of(rows, places, gates);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    const at::Tensor &rows = saved[0], &places = saved[1], &gates = saved[2];
+    const c10::cuda::CUDAGuard guard(places.device());
+    const at::Tensor grad = grads[0].contiguous();
+    const int64_t T = places.size(0), k = places.size(1);
+    at::Tensor row_grads, gate_grads;
+    if (ctx->needs_input_grad(0)) row_grads = like_rows(grad, T * k);
+    if (ctx->needs_input_grad(2)) gate_grads = empty({T, k}, gates.scalar_type(), gates.device());
+    done(brt_unsort_cells_backward(
+        grad.data_ptr(), data_or_null(rows), static_cast<const int32_t*>(places.data_ptr()),
+        gates.data_ptr(), data_or_null(row_grads), data_or_null(gate_grads), T, (int)k,
+        grad.numel() / T, dtype_of(grad), dtype_of(gates), stream_of(grad)));
+    return once({row_grads, at::Tensor(), gate_grads});
+  }
+};
+
+// order_picks(picks, path_num) -> (places, loads)
+PyObject* order_picks(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    if (n != 2 || modes_active()) return nullptr;
+    const at::Tensor* picks = plain(a[0]);
+    if (picks == nullptr || picks->dim() != 2 || !picks->is_contiguous() || picks->numel() == 0 ||
+        !Place::of(*picks) ||
+        (picks->scalar_type() != at::kInt && picks->scalar_type() != at::kLong))
+      return nullptr;
+    const long paths = PyLong_AsLong(a[1]);
+    if (PyErr_Occurred()) {
+      PyErr_Clear();
+      return nullptr;
+    }
+    if (paths < 1 || paths > 1024) return nullptr;
+    Memory memory;
+    const Place p(*picks);
+    const int64_t T = picks->size(0), k = picks->size(1);
+    const bool wide = picks->scalar_type() == at::kLong;
+    const void* const from = memory.of(picks);
+    at::Tensor places, loads;
+    int rc;
+    {
+      const Unlocked unlocked;
+      places = empty({T, k}, at::kInt, p.device);
+      loads = empty({paths}, at::kInt, p.device);
+      const int64_t bytes = (int64_t)brt_pick_order_scratch_bytes(T * k, (int)paths);
+      at::Tensor scratch;
+      if (bytes > 0) scratch = empty({bytes}, at::kByte, p.device);
+      rc = brt_order_picks(from, wide, T * k, (int)paths,
+                           static_cast<int32_t*>(places.data_ptr()),
+                           static_cast<int32_t*>(loads.data_ptr()), data_or_null(scratch),
+                           (size_t)bytes, p.handle());
+    }
+    if (rc != BRT_OK) return nullptr;
+    return Py_BuildValue("(NN)", THPVariable_Wrap(places), THPVariable_Wrap(loads));
+  });
+}
+
+// sort_cells(in_data, places) -> rows
+PyObject* sort_cells(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    if (n != 2 || modes_active()) return nullptr;
+    const at::Tensor *x = plain(a[0]), *places = plain(a[1]);
+    if (x == nullptr || x->dim() < 1 || !x->is_contiguous() || x->numel() == 0 ||
+        dtype_of(*x) < 0 || !Place::of(*x) || !is_places(places) || !same_device(*x, places) ||
+        x->size(0) != places->size(0))
+      return nullptr;
+    const at::Tensor cells = *x, at_rows = *places;  // kept while other threads run
+    const bool grad = wants_grad(x);
+    at::Tensor rows;
+    {
+      const Unlocked unlocked;
+      rows = grad ? SortCells::apply(cells, at_rows) : sorted_rows(cells, at_rows);
+    }
+    return THPVariable_Wrap(rows);
+  });
+}
+
+// sort_cells_fp8(in_data, places) -> (codes, scales)
+PyObject* sort_cells_fp8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    if (n != 2 || modes_active()) return nullptr;
+    const at::Tensor *x = plain(a[0]), *places = plain(a[1]);
+    if (x == nullptr || x->dim() != 2 || !x->is_contiguous() || x->numel() == 0 ||
+        dtype_of(*x) < 0 || x->size(1) % 16 != 0 || wants_grad(x) || !Place::of(*x) ||
+        !is_places(places) || !same_device(*x, places) || x->size(0) != places->size(0))
+      return nullptr;
+    Memory memory;
+    const Place p(*x);
+    const int64_t T = x->size(0), k = places->size(1), width = x->size(1);
+    const int dtype = dtype_of(*x);
+    const void* const from = memory.of(x);
+    if (reinterpret_cast<uintptr_t>(from) % 16 != 0) return nullptr;
+    const int32_t* const at_rows = memory.ints(places);
+    at::Tensor codes, scales;
+    int rc;
+    {
+      const Unlocked unlocked;
+      codes = empty({T * k, width}, at::kFloat8_e4m3fn, p.device);
+      scales = empty({(width + 127) / 128, T * k}, at::kFloat, p.device);
+      rc = brt_sort_cells_fp8(from, at_rows, codes.data_ptr(),
+                              static_cast<float*>(scales.data_ptr()), T, (int)k, width, dtype,
+                              p.handle());
+      scales = scales.t();
+    }
+    if (rc != BRT_OK) return nullptr;
+    return Py_BuildValue("(NN)", THPVariable_Wrap(codes), THPVariable_Wrap(scales));
+  });
+}
+
+// unsort_cells(rows, places, gates | None) -> cells
+PyObject* unsort_cells(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    if (n != 3 || modes_active()) return nullptr;
+    const at::Tensor *x = plain(a[0]), *places = plain(a[1]), *weights = nullptr;
+    if (x == nullptr || x->dim() < 1 || !x->is_contiguous() || x->numel() == 0 ||
+        dtype_of(*x) < 0 || !Place::of(*x) || !is_places(places) || !same_device(*x, places) ||
+        x->size(0) != places->numel())
+      return nullptr;
+    if (a[2] != Py_None) {
+      weights = plain(a[2]);
+      if (weights == nullptr || !weights->is_contiguous() || weights->sizes() != places->sizes() ||
+          !same_device(*x, weights) ||
+          (weights->scalar_type() != at::kFloat && weights->scalar_type() != x->scalar_type()))
+        return nullptr;
+    }
+    const at::Tensor rows = *x, at_rows = *places;  // kept while other threads run
+    const at::Tensor gates = weights != nullptr ? *weights : at::Tensor();
+    const bool grad = wants_grad(x) || wants_grad(weights);
+    at::Tensor cells;
+    {
+      const Unlocked unlocked;
+      cells = !grad              ? cells_of(rows, at_rows, gates)
+              : gates.defined() ? UnsortCells::apply(rows, at_rows, gates)
+                                : SumCells::apply(rows, at_rows);
+    }
+    return THPVariable_Wrap(cells);
+  });
+}
+
 PyMethodDef methods[] = {
     {"scan", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(scan)), METH_FASTCALL, nullptr},
     {"route_scores", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(route_scores)),
@@ -414,6 +637,14 @@ PyMethodDef methods[] = {
      nullptr},
     {"combine", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(combine)), METH_FASTCALL,
      nullptr},
+    {"order_picks", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(order_picks)),
+     METH_FASTCALL, nullptr},
+    {"sort_cells", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(sort_cells)),
+     METH_FASTCALL, nullptr},
+    {"sort_cells_fp8", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(sort_cells_fp8)),
+     METH_FASTCALL, nullptr},
+    {"unsort_cells", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(unsort_cells)),
+     METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host_ops", nullptr, -1, methods,
                       nullptr, nullptr, nullptr, nullptr};

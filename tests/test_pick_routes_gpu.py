@@ -302,3 +302,85 @@ def test_captured_training_pass():
     torch.cuda.synchronize()
     for a, b in zip(got, step()):
         assert torch.equal(a, b)
+
+
+@pytest.fixture(params=["native", "python"])
+def host_side(request, monkeypatch):
+    """The operators with their native host side, and with the Python that takes what it declines."""
+    from brainstorm_b200 import _lib
+
+    if request.param == "python":
+        monkeypatch.setattr(_lib, "_host", _lib._DeclinesAll())
+    return request.param
+
+
+@pytest.mark.parametrize("gate_type", [None, torch.float32, torch.bfloat16])
+def test_both_host_sides(host_side, gate_type):
+    from brainstorm_b200._C import router as R
+
+    torch.manual_seed(4)
+    T, k, E, d = 90, 3, 11, 160
+    picks = torch.tensor(make_picks(T, k, E, "dropped"), device="cuda")
+    places, loads = R.order_picks(picks, E)
+    want, want_loads = order_by_hand(picks.cpu().numpy(), E)
+    assert np.array_equal(places.cpu().numpy(), want)
+    assert np.array_equal(loads.cpu().numpy(), want_loads)
+    x = torch.randn(T, d, device="cuda").bfloat16().requires_grad_()
+    gates = None if gate_type is None else \
+        torch.rand(T, k, device="cuda").to(gate_type).requires_grad_()
+    rows = R.sort_cells(x, places)
+    out = R.unsort_cells(rows, places, gates)
+    gy = torch.randn(T, d, device="cuda").bfloat16()
+    leaves = [x] if gates is None else [x, gates]
+    grads = torch.autograd.grad(out, leaves, gy)
+    live = (places >= 0).float()
+    weight = live if gates is None else live * gates.detach().float()
+    # sums of up to 3 products of bf16 values: the products are exact in fp32 but for fp32 gates
+    # (2^-24), the sums are off by 2^-23 of their terms, and each result is rounded to bf16: twice
+    # on the way back
+    size = weight.sum(1, keepdim=True)
+    plain = x.detach().float() * size
+    assert bool(((out.detach().float() - plain).abs() <= 2.0 ** -8 * plain.abs() * 1.01).all())
+    plain = gy.float() * size
+    tol = 2.0 ** -8 * 2.01 * (gy.float().abs() * size) + 1e-30
+    assert bool(((grads[0].float() - plain).abs() <= tol).all())
+    if gates is not None:
+        dots = (gy.double() * x.detach().double()).sum(1, keepdim=True) * live
+        size = (gy.double() * x.detach().double()).abs().sum(1, keepdim=True)
+        half = torch.finfo(gate_type).eps / 2
+        assert bool(((grads[1].double() - dots).abs()
+                     <= (d + 5) * 2.0 ** -24 * size + half * dots.abs() * 1.01).all())
+    codes, scales = R.sort_cells_fp8(x.detach(), places)
+    assert codes.shape == (T * k, d) and scales.stride() == (1, T * k)
+    # a gradient that comes expanded, and one of the leaves alone
+    (g,) = torch.autograd.grad(R.sort_cells(x, places).sum(), (x,))
+    assert torch.equal(g.float(), live.sum(1, keepdim=True).expand(T, d))
+    if gates is not None:
+        out = R.unsort_cells(rows.detach(), places, gates)
+        (g,) = torch.autograd.grad(out, (gates,), gy)
+        assert torch.equal(g, grads[1])
+
+
+def test_second_gradients_are_refused(host_side):
+    from brainstorm_b200._C import router as R
+
+    places, _ = R.order_picks(torch.tensor([[0, 1], [1, 0]], device="cuda"), 2)
+    x = torch.randn(2, 16, device="cuda", requires_grad=True)
+    gates = torch.rand(2, 2, device="cuda", requires_grad=True)
+    out = R.unsort_cells(R.sort_cells(x, places), places, gates)
+    gx, gg = torch.autograd.grad(out.square().sum(), (x, gates), create_graph=True)
+    assert bool(torch.isfinite(gx).all()) and bool(torch.isfinite(gg).all())
+    with pytest.raises(RuntimeError, match="differentia"):
+        torch.autograd.grad(gg.sum(), x)
+
+
+def test_an_edited_input_is_noticed_by_the_backward_pass(host_side):
+    from brainstorm_b200._C import router as R
+
+    places, _ = R.order_picks(torch.tensor([[0, 1], [1, 0]], device="cuda"), 2)
+    rows = torch.randn(4, 16, device="cuda")
+    gates = torch.rand(2, 2, device="cuda", requires_grad=True)
+    out = R.unsort_cells(rows, places, gates)
+    rows.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
