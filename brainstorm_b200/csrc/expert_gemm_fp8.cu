@@ -17,12 +17,19 @@
 // The scales are any fp32 numbers, which the tensor cores cannot apply: each block of 128 along
 // K is one fresh accumulation in tensor memory (4 MMAs of K = 32), which the accumulating warps
 // multiply by rs * ws and add to fp32 registers while the next block is being multiplied into
-// the other half of tensor memory.  The rows are the M operand: a CTA pair (cta_group::2) computes
-// 256 rows x 256 features, 128 rows (the lanes of tensor memory) in each CTA, and a thread holds
-// 128 features of ONE row, a scale block: it needs one scale per block of K.  (With the weights as
-// M, as in the bf16 kernel, no row is computed for padding, but a thread needs the scales of 128
-// rows; the shared-memory reads for them made every size slower: 1024 rows per expert, 4096 ->
-// 4096, 551 us against 322; 64 rows per expert, 102 against 82; a row each, the same.)
+// the other half of tensor memory.  The rows are the M operand, 128 (the lanes of tensor memory)
+// per CTA, and 256 features the N operand: a thread holds 128 features of ONE row, a scale block,
+// and needs one scale per block of K.  (With the weights as M, as in the bf16 kernel, no row is
+// computed for padding, but a thread needs the scales of 128 rows; the shared-memory reads for
+// them made every size slower: 1024 rows per expert, 4096 -> 4096, 551 us against 322; 64 rows per
+// expert, 102 against 82.)
+// Two forms: CTA pairs (cta_group::2, 256 rows x 256 features, half of the features fetched by
+// each) for many rows, single CTAs (128 x 256) for few: there the work on a block of K takes as
+// long as ever for however few rows, and a CTA gets twice the weights through in that time.
+//
+// What bounds it: with many rows the accumulating warps (65536 rows in 32 experts, 4096 -> 4096:
+// 1065 us, 2065 TFLOP/s; 790 us without them) and under a sustained load the 1000 W limit; with few
+// the reading of the weights (a row in each of 64 experts, 2048 -> 4096: 97 us, 5.5 TB/s).
 // Roles inside a CTA (384 threads):
 //   warp 0     TMA loads into a shared-memory ring, 128 bytes of K per slot and row (128-byte
 //              swizzle): its 128 features, and of its 128 rows those that exist, in one box of
@@ -49,16 +56,28 @@ constexpr int kBN = 256;      // features per tile
 constexpr int kBoxStep = 32;  // the rows come in one box of 32, 64, 96 or 128
 constexpr int kBoxSizes = 4;
 constexpr int kMmaK = 32;
-constexpr int kStages = 6;
+// ring slots: 32 KB each with a pair, 48 KB without
+template <int kPair>
+constexpr int kStages = kPair == 2 ? 6 : 4;
 constexpr int kScaleSlots = 4;
 constexpr int kAccWarps = 8;
 constexpr int kFirstScaleWarp = 2;
 constexpr int kFirstAccWarp = 4;  // warps are given registers by fours
 constexpr int kThreads = 32 * (kFirstAccWarp + kAccWarps);
 // The block starts with 168 registers a thread.  The accumulators alone are 128 of an
-// accumulating thread's, so the other four warps hand over what they do not need.
-constexpr int kFewRegisters = 88, kManyRegisters = 208;
-static_assert(128 * kFewRegisters + 32 * kAccWarps * kManyRegisters == kThreads * 168, "registers");
+// accumulating thread's, so the other four warps hand over what they do not need (the splits that
+// were fastest: pairs 5 to 10 % slower with the other's, single CTAs 10 %).
+template <int kPair>
+constexpr int kFewRegisters = kPair == 2 ? 88 : 56;
+template <int kPair>
+constexpr int kManyRegisters = kPair == 2 ? 208 : 224;
+static_assert(128 * kFewRegisters<1> + 32 * kAccWarps * kManyRegisters<1> == kThreads * 168 &&
+              128 * kFewRegisters<2> + 32 * kAccWarps * kManyRegisters<2> == kThreads * 168,
+              "registers");
+// Rows per expert on average up to which single CTAs are taken.  16 experts, 4096 -> 4096: 32 rows
+// 64 us against 80 with pairs, 128 rows 82 against 84, 256 rows 125 against 116, 1024 rows 359
+// against 319; a row in each of 64 experts, 2048 -> 4096: 97 against 139.
+constexpr int kSingleRows = 192;
 constexpr uint32_t kRowBytes = kBK;
 constexpr uint32_t kTileBytes = kBM * kRowBytes;
 
@@ -84,21 +103,31 @@ struct Fp8Args {
   int zero_unused;
 };
 
-// kind::f8f6f4: fp32 accumulators, e4m3 x e4m3, both operands K-major, M = 256 and N = 256.
-constexpr uint32_t kInstruction =
-    (1u << 4) | ((uint32_t)(kBN >> 3) << 17) | ((uint32_t)(2 * kBM >> 4) << 24);
+// kind::f8f6f4: fp32 accumulators, e4m3 x e4m3, both operands K-major, N = 256.
+template <int kPair>
 __device__ __forceinline__ void mma_fp8(uint32_t tmem_d, uint64_t a, uint64_t b,
                                         uint32_t accumulate) {
-  asm volatile(
-      "{\n"
-      ".reg .pred p;\n"
-      "setp.ne.b32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n"
-      "}\n" ::"r"(tmem_d),
-      "l"(a), "l"(b), "r"(kInstruction), "r"(accumulate)
-      : "memory");
+  constexpr uint32_t kInstruction =
+      (1u << 4) | ((uint32_t)(kBN >> 3) << 17) | ((uint32_t)(kPair * kBM >> 4) << 24);
+  if constexpr (kPair == 2)
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n"
+        "}\n" ::"r"(tmem_d),
+        "l"(a), "l"(b), "r"(kInstruction), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n"
+        "}\n" ::"r"(tmem_d),
+        "l"(a), "l"(b), "r"(kInstruction), "r"(accumulate)
+        : "memory");
 }
-
 // acc += v * scale for 32 columns, two at a time.  The empty statements keep the additions in
 // front of the loads that follow: the compiler would move them behind, and then hold more columns
 // in registers than there are.
@@ -114,12 +143,13 @@ __device__ __forceinline__ void add_scaled(float2* acc, const uint32_t (&v)[32],
                       "+f"(acc[i + 3].y));
 }
 
+template <int kPair>
 struct alignas(1024) Fp8Smem {
-  unsigned char a[kStages][kTileBytes];  // 128 rows
-  unsigned char b[kStages][kTileBytes];  // 128 features: half of the pair's
+  unsigned char a[kStages<kPair>][kTileBytes];               // 128 rows
+  unsigned char b[kStages<kPair>][kBN / kPair * kRowBytes];  // half of a pair's features, or all
   unsigned char turn[kAccWarps][32 * 64];
-  uint64_t full[kStages];
-  uint64_t empty[kStages];
+  uint64_t full[kStages<kPair>];
+  uint64_t empty[kStages<kPair>];
   uint64_t acc_full[2];
   uint64_t acc_empty[2];
   uint64_t scale_full[kScaleSlots][2];  // [slot][scale block of the tile]
@@ -129,23 +159,25 @@ struct alignas(1024) Fp8Smem {
   uint32_t tmem_base;
   ExpertTable table;
 };
-static_assert(sizeof(Fp8Smem) + 1024 <= 232448, "shared memory of an SM");
+static_assert(sizeof(Fp8Smem<1>) + 1024 <= 232448 && sizeof(Fp8Smem<2>) + 1024 <= 232448,
+              "shared memory of an SM");
 
 struct TileAt {
   int expert, n_tile;
   int row0, rows;  // within the expert
 };
+template <int kPair>
 __device__ __forceinline__ TileAt tile_at(const ExpertTable& table, const Fp8Args& g, int t) {
   TileAt at;
   at.expert = expert_of_tile(table, g.experts, t);
   const int local = t - table.first_tile[at.expert];
   const int part = local / g.n_tiles;
   at.n_tile = local - part * g.n_tiles;
-  at.row0 = part * 2 * kBM;
-  at.rows = min(2 * kBM, table.load[at.expert] - at.row0);
+  at.row0 = part * kPair * kBM;
+  at.rows = min(kPair * kBM, table.load[at.expert] - at.row0);
   return at;
 }
-// Boxes of 32 rows that CTA `rank` of the pair fetches for a tile.
+// Boxes of 32 rows that CTA `rank` fetches for a tile.
 __device__ __forceinline__ int boxes_of(int rows, int rank) {
   const int mine = min(kBM, rows - rank * kBM);
   return mine > 0 ? (mine + kBoxStep - 1) / kBoxStep : 0;
@@ -167,30 +199,34 @@ __device__ __forceinline__ void zero_unused_rows(const ExpertTable& table, const
   }
 }
 
+template <int kPair>
 __global__ void __launch_bounds__(kThreads, 1)
 expert_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w,
                        const __grid_constant__ RowMaps map_r, const Fp8Args g) {
   extern __shared__ __align__(1024) unsigned char s_raw[];
-  Fp8Smem& s = *reinterpret_cast<Fp8Smem*>((reinterpret_cast<uintptr_t>(s_raw) + 1023) &
-                                           ~static_cast<uintptr_t>(1023));
+  constexpr int kRing = kStages<kPair>;
+  Fp8Smem<kPair>& s = *reinterpret_cast<Fp8Smem<kPair>*>(
+      (reinterpret_cast<uintptr_t>(s_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  const int rank = (int)cluster_rank();
-  const int group = blockIdx.x / 2;
-  const int groups = gridDim.x / 2;
+  const int rank = kPair == 2 ? (int)cluster_rank() : 0;
+  const int group = blockIdx.x / kPair;
+  const int groups = gridDim.x / kPair;
 
   if (warp == 0) {
     const int n_tiles = g.n_tiles;
     fill_expert_table(s.table, g.loads, g.experts, g.max_path_load, g.total_rows,
-                      [n_tiles](int load) { return (load + 2 * kBM - 1) / (2 * kBM) * n_tiles; });
+                      [n_tiles](int load) {
+                        return (load + kPair * kBM - 1) / (kPair * kBM) * n_tiles;
+                      });
     if (lane == 0) {
-      for (int i = 0; i < kStages; i++) {
+      for (int i = 0; i < kRing; i++) {
         mbar_init(&s.full[i], 1);
         mbar_init(&s.empty[i], 1);
       }
       for (int i = 0; i < 2; i++) {
         mbar_init(&s.acc_full[i], 1);
-        mbar_init(&s.acc_empty[i], kAccWarps * 2);
+        mbar_init(&s.acc_empty[i], kAccWarps * kPair);
       }
       for (int i = 0; i < 2 * kScaleSlots; i++) {
         mbar_init(&s.scale_full[i >> 1][i & 1], 32);
@@ -199,41 +235,46 @@ expert_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w,
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
   }
-  if (warp == 1) tmem_alloc<2>(&s.tmem_base);
+  if (warp == 1) tmem_alloc<kPair>(&s.tmem_base);
   tcgen05_before_sync();
   __syncthreads();
-  group_sync<2>();  // the peer's barriers exist
+  group_sync<kPair>();  // the peer's barriers exist
   tcgen05_after_sync();
   const uint32_t tmem = s.tmem_base;
   const int total_tiles = s.table.first_tile[g.experts];
   bool failed = false;
 
   if (warp < kFirstAccWarp) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegisters));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegisters<kPair>));
     if (warp == 0) {
       int slot = 0;
       uint32_t phase = 0;
       for (int t = group; t < total_tiles && !failed; t += groups) {
-        const TileAt at = tile_at(s.table, g, t);
+        const TileAt at = tile_at<kPair>(s.table, g, t);
         const int boxes = boxes_of(at.rows, rank);
         const CUtensorMap* const map_box = &map_r.box[boxes > 0 ? boxes - 1 : 0];
         const int row0 = s.table.row_base[at.expert] + at.row0 + rank * kBM;
         const int feature0 = at.n_tile * kBN + rank * kBM;
         const int blocks = min(2, g.n_blocks - at.n_tile * 2);  // the last tile may have but one
         const uint32_t bytes =
-            (uint32_t)(boxes_of(at.rows, 0) + boxes_of(at.rows, 1)) * kBoxStep * kRowBytes +
+            (uint32_t)(boxes_of(at.rows, 0) + (kPair == 2 ? boxes_of(at.rows, 1) : 0)) * kBoxStep *
+                kRowBytes +
             (uint32_t)blocks * kTileBytes;
         for (int kb = 0; kb < g.k_blocks; kb++) {
           if (!mbar_wait(&s.empty[slot], phase ^ 1)) { failed = true; break; }
           if (elect_one()) {
             if (rank == 0) mbar_expect_tx(&s.full[slot], bytes);  // of both CTAs
-            const uint32_t bar = map_to_cta(&s.full[slot], 0);
+            const uint32_t bar =
+                kPair == 2 ? map_to_cta(&s.full[slot], 0) : smem_u32(&s.full[slot]);
             if (rank < blocks)
-              tma_load_3d<2>(s.b[slot], &map_w, bar, kb * kBK, feature0, at.expert);
-            if (boxes > 0) tma_load_2d<2>(s.a[slot], map_box, bar, kb * kBK, row0);
+              tma_load_3d<kPair>(s.b[slot], &map_w, bar, kb * kBK, feature0, at.expert);
+            if (kPair == 1 && blocks == 2)
+              tma_load_3d<kPair>(s.b[slot] + kTileBytes, &map_w, bar, kb * kBK, feature0 + kBM,
+                                 at.expert);
+            if (boxes > 0) tma_load_2d<kPair>(s.a[slot], map_box, bar, kb * kBK, row0);
           }
           __syncwarp();
-          if (++slot == kStages) { slot = 0; phase ^= 1; }
+          if (++slot == kRing) { slot = 0; phase ^= 1; }
         }
       }
       // copies still in flight land before the CTA's shared memory is given back
@@ -256,12 +297,12 @@ expert_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w,
               const uint32_t d = tmem + (uint32_t)buf * kBN;
 #pragma unroll
               for (int k = 0; k < kBK / kMmaK; k++)  // 32 bytes further along the swizzled row
-                mma_fp8(d, da + 2 * k, db + 2 * k, k != 0);
-              umma_commit<2>(&s.empty[slot]);
-              umma_commit<2>(&s.acc_full[buf]);
+                mma_fp8<kPair>(d, da + 2 * k, db + 2 * k, k != 0);
+              umma_commit<kPair>(&s.empty[slot]);
+              umma_commit<kPair>(&s.acc_full[buf]);
             }
             __syncwarp();
-            if (++slot == kStages) { slot = 0; phase ^= 1; }
+            if (++slot == kRing) { slot = 0; phase ^= 1; }
             buf ^= 1;
             if (buf == 0) buf_phase ^= 1;
           }
@@ -272,7 +313,7 @@ expert_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w,
       int slot = 0;
       uint32_t phase = 0;
       for (int t = group; t < total_tiles && !failed; t += groups) {
-        const TileAt at = tile_at(s.table, g, t);
+        const TileAt at = tile_at<kPair>(s.table, g, t);
         const int feature_block = min(at.n_tile * 2 + half, g.n_blocks - 1);
         const float* const ws =
             g.weight_scales + ((long long)at.expert * g.n_blocks + feature_block) * g.k_blocks;
@@ -295,18 +336,19 @@ expert_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w,
       asm volatile("cp.async.wait_all;" ::: "memory");
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegisters));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegisters<kPair>));
     const int quarter = warp & 3;  // the 32 lanes of tensor memory that this warp may read
     const int half = (warp - kFirstAccWarp) / 4;  // of the tile's features: one scale block
     unsigned char* const turn = s.turn[warp - kFirstAccWarp];
     const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * kBM);
-    const uint32_t handed_back = map_to_cta(&s.acc_empty[0], 0);
+    const uint32_t handed_back =
+        kPair == 2 ? map_to_cta(&s.acc_empty[0], 0) : smem_u32(&s.acc_empty[0]);
     const float* const row_scale = &s.row_scale[0][half][quarter * 32 + lane];
     const int row0 = rank * kBM + quarter * 32;  // of the tile
     int buf = 0, slot = 0;
     uint32_t buf_phase = 0, phase = 0;
     for (int t = group; t < total_tiles && !failed; t += groups) {
-      const TileAt at = tile_at(s.table, g, t);
+      const TileAt at = tile_at<kPair>(s.table, g, t);
       const int feature0 = at.n_tile * kBN + half * kBM;
       const int rows = feature0 < g.N ? at.rows - row0 : 0;  // of this warp
       float2 acc[kBM / 2];
@@ -379,35 +421,36 @@ expert_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w,
   __syncwarp();
 
   tcgen05_before_sync();
-  group_sync<2>();  // nobody leaves while the peer may still signal its barriers
+  group_sync<kPair>();  // nobody leaves while the peer may still signal its barriers
   tcgen05_after_sync();
-  if (warp == 1) tmem_free<2>(tmem);
+  if (warp == 1) tmem_free<kPair>(tmem);
 }
 
+template <int kPair>
 int launch_fp8(const CUtensorMap& map_w, const RowMaps& map_r, const Fp8Args& g, cudaStream_t st) {
-  const size_t smem = sizeof(Fp8Smem) + 1024;
+  const size_t smem = sizeof(Fp8Smem<kPair>) + 1024;
   static thread_local int configured_device = -1;
   int dev = 0;
   BRT_CUDA_TRY(cudaGetDevice(&dev));
   if (configured_device != dev) {
-    BRT_CUDA_TRY(cudaFuncSetAttribute(expert_gemm_fp8_kernel,
+    BRT_CUDA_TRY(cudaFuncSetAttribute(expert_gemm_fp8_kernel<kPair>,
                                       cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     configured_device = dev;
   }
   cudaLaunchAttribute cluster;
   cluster.id = cudaLaunchAttributeClusterDimension;
-  cluster.val.clusterDim.x = 2;
+  cluster.val.clusterDim.x = kPair;
   cluster.val.clusterDim.y = 1;
   cluster.val.clusterDim.z = 1;
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3((unsigned)(sm_count() / 2 * 2));
+  config.gridDim = dim3((unsigned)(sm_count() / kPair * kPair));
   config.blockDim = dim3(kThreads);
   config.dynamicSmemBytes = smem;
   config.stream = st;
   config.attrs = &cluster;
   config.numAttrs = 1;
   const KernelTimer timer("expert_gemm_fp8_kernel", st);
-  BRT_CUDA_TRY(cudaLaunchKernelEx(&config, expert_gemm_fp8_kernel, map_w, map_r, g));
+  BRT_CUDA_TRY(cudaLaunchKernelEx(&config, expert_gemm_fp8_kernel<kPair>, map_w, map_r, g));
   note_launch();
   return BRT_OK;
 }
@@ -446,7 +489,9 @@ BRT_API int brt_grouped_expert_gemm_fp8(const void* rows, const float* row_scale
               "too many features");
   const int n_blocks = (int)((out_features + kBM - 1) / kBM);
   const int n_tiles = (n_blocks + 1) / 2;
-  BRT_REQUIRE((total_rows / (2 * kBM) + path_num) * (int64_t)n_tiles < (1LL << 31) - 1024,
+  const int64_t mean_rows = max_path_load != 0 ? max_path_load : total_rows / path_num;
+  const bool pair = mean_rows > kSingleRows;
+  BRT_REQUIRE((total_rows / kBM + path_num) * (int64_t)n_tiles < (1LL << 31) - 1024,
               "more tiles than 32 bits count");
   EncodeTiledFn encode = encode_tiled();
   if (encode == nullptr)
@@ -499,7 +544,7 @@ BRT_API int brt_grouped_expert_gemm_fp8(const void* rows, const float* row_scale
   g.relu = relu != 0;
   g.zero_unused = zero_unused != 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return launch_fp8(map_w, map_r, g, st);
+  return pair ? launch_fp8<2>(map_w, map_r, g, st) : launch_fp8<1>(map_w, map_r, g, st);
 }
 
 }  // extern "C"
