@@ -44,6 +44,7 @@ constexpr int kSumWarps = 8;
 constexpr int kThreads = 32 * (kFirstSumWarp + kSumWarps);
 constexpr int kFewRegisters = 88, kManyRegisters = 208;
 static_assert(128 * kFewRegisters + 32 * kSumWarps * kManyRegisters == kThreads * 168, "registers");
+constexpr int kMaxSorted = 256;
 constexpr int kChunk = 16;     // ring slots (1024 rows) per accumulator
 template <int kPair>
 constexpr int kStages = kPair == 2 ? 6 : 4;
@@ -92,6 +93,7 @@ struct alignas(1024) WgradSmem {
   uint64_t acc_empty[2];
   uint32_t tmem_base;
   ExpertTable table;
+  int order[kMaxExperts];  // experts by descending load
 };
 
 struct WgradTile {
@@ -99,13 +101,19 @@ struct WgradTile {
   int row0, load;
   int blocks;  // ring slots
 };
+// The tiles of the largest experts come first, and are dealt out to and fro.
+__device__ __forceinline__ int wgrad_turn(int round, int group, int groups) {
+  return round * groups + (round & 1 ? groups - 1 - group : group);
+}
 template <int kPair>
-__device__ __forceinline__ WgradTile wgrad_tile(const ExpertTable& table, const WgradArgs& g,
+__device__ __forceinline__ WgradTile wgrad_tile(const WgradSmem<kPair>& s, const WgradArgs& g,
                                                 int t) {
   WgradTile at;
+  const ExpertTable& table = s.table;
   const int per = g.m_tiles * g.n_tiles;
-  at.expert = t / per;
-  const int local = t - at.expert * per;
+  const int which = t / per;
+  at.expert = s.order[which];
+  const int local = t - which * per;
   const int part = local / g.m_tiles;
   at.n0 = (local - part * g.m_tiles) * kBM * kPair;
   at.k0 = part * g.width;
@@ -165,6 +173,21 @@ expert_wgrad_kernel(const __grid_constant__ CUtensorMap map_g,
     }
   }
   if (warp == 1) tmem_alloc<kPair>(&s.tmem_base);
+  __syncthreads();
+  // A tile takes as long as its expert has rows, so uneven experts are dealt out by load.  All
+  // pairs are compared; beyond kMaxSorted experts that would take longer than it gains.
+  for (int e = threadIdx.x; e < g.experts; e += kThreads) {
+    int rank = e;
+    if (g.experts <= kMaxSorted) {
+      rank = 0;
+      const int mine = s.table.load[e];
+      for (int j = 0; j < g.experts; j++) {
+        const int other = s.table.load[j];
+        rank += other > mine || (other == mine && j < e);
+      }
+    }
+    s.order[rank] = e;
+  }
   tcgen05_before_sync();
   __syncthreads();
   group_sync<kPair>();
@@ -179,8 +202,9 @@ expert_wgrad_kernel(const __grid_constant__ CUtensorMap map_g,
       uint32_t phase = 0;
       const int b_boxes = (half + kBoxFeatures - 1) / kBoxFeatures;
       const uint32_t bytes = (uint32_t)(kABoxes + b_boxes) * kBoxBytes;
-      for (int t = group; t < total_tiles && !failed; t += groups) {
-        const WgradTile at = wgrad_tile<kPair>(s.table, g, t);
+      for (int round = 0, t = group; t < total_tiles && !failed;
+         t = wgrad_turn(++round, group, groups)) {
+        const WgradTile at = wgrad_tile<kPair>(s, g, t);
         const int n0 = at.n0 + (int)rank * kBM;
         const int k0 = at.k0 + (int)rank * half;
         for (int i = 0; i < at.blocks; i++) {
@@ -217,8 +241,9 @@ expert_wgrad_kernel(const __grid_constant__ CUtensorMap map_g,
         int slot = 0, acc = 0;
         uint32_t phase = 0, acc_phase = 0;
         const uint32_t idesc = wgrad_idesc<kPair>(g.width);
-        for (int t = group; t < total_tiles && !failed; t += groups) {
-          const WgradTile at = wgrad_tile<kPair>(s.table, g, t);
+        for (int round = 0, t = group; t < total_tiles && !failed;
+         t = wgrad_turn(++round, group, groups)) {
+          const WgradTile at = wgrad_tile<kPair>(s, g, t);
           for (int i = 0; i < at.blocks; i++) {
             if ((i % kChunk == 0 && !mbar_wait(&s.acc_empty[acc], acc_phase ^ 1)) ||
                 !mbar_wait(&s.full[slot], phase)) {
@@ -249,8 +274,9 @@ expert_wgrad_kernel(const __grid_constant__ CUtensorMap map_g,
       int slot = 0;            // of the next tile's first block
       uint32_t phases = 0;     // one bit per tail barrier
       const int b_boxes = (half + kBoxFeatures - 1) / kBoxFeatures;
-      for (int t = group; t < total_tiles && !failed; t += groups) {
-        const WgradTile at = wgrad_tile<kPair>(s.table, g, t);
+      for (int round = 0, t = group; t < total_tiles && !failed;
+         t = wgrad_turn(++round, group, groups)) {
+        const WgradTile at = wgrad_tile<kPair>(s, g, t);
         const int rows = at.load % kBR;
         if (rows != 0) {
           const int last = (slot + at.blocks - 1) % kRing;
@@ -284,8 +310,9 @@ expert_wgrad_kernel(const __grid_constant__ CUtensorMap map_g,
     constexpr int kSize = kFloatOut ? 4 : 2;
     int acc = 0;
     uint32_t acc_phase = 0;
-    for (int t = group; t < total_tiles && !failed; t += groups) {
-      const WgradTile at = wgrad_tile<kPair>(s.table, g, t);
+    for (int round = 0, t = group; t < total_tiles && !failed;
+         t = wgrad_turn(++round, group, groups)) {
+      const WgradTile at = wgrad_tile<kPair>(s, g, t);
       float sum[kBN / 2];
 #pragma unroll
       for (int i = 0; i < kBN / 2; i++) sum[i] = 0.f;
