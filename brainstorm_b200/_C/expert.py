@@ -121,6 +121,9 @@ def quantize_rows(rows: torch.Tensor):
     value is ``code * scale``.  ``scale = max(max |x|, 2**-100) / 448``.  The scales of a block lie
     together for all rows (strides (1, L)), as the products read them.  A NaN stays NaN by itself;
     an infinity makes its block's scale infinite.  The width must be a multiple of 16."""
+    done = _lib.host_ops().quantize_rows(rows)
+    if done is not None:
+        return done
     if not rows.is_cuda:
         raise RuntimeError("rows must be a CUDA tensor")
     if rows.dtype not in _DT:
@@ -181,6 +184,13 @@ def grouped_expert_linear_fp8(rows: torch.Tensor, row_scales: torch.Tensor,
     numbers; sums run in fp32.  Returns [L, out] bf16.  Rows beyond an expert's load are left
     unwritten, or set to zero with ``zero_unused``.  ``in`` and ``out`` are multiples of 16.  The
     other arguments are those of ``grouped_expert_linear``."""
+    word = _error_words.get(rows.get_device())
+    if word is not None and (not max_path_padding or max_path_load > 0):
+        done = _lib.host_ops().grouped_expert_linear_fp8(
+            rows, row_scales, weights, weight_scales, loads,
+            max_path_load if max_path_padding else 0, relu, out, zero_unused, word)
+        if done is not None:
+            return done
     for t in (rows, row_scales, weights, weight_scales, loads):
         if not t.is_cuda:
             raise RuntimeError("rows, weights, their scales and loads must be CUDA tensors")
@@ -225,6 +235,14 @@ def grouped_expert_weight_grad(grads: torch.Tensor, rows: torch.Tensor, loads: t
     (what went into it), laid out and counted by ``loads`` as for ``grouped_expert_linear``.
     Returns [E, out, in] in ``dtype`` (bf16 or fp32), fp32 sums rounded once; zeros for an expert
     without rows.  Rows beyond an expert's load are not looked at.  Multiples of 16."""
+    word = _error_words.get(rows.get_device())
+    if word is not None and (not max_path_padding or max_path_load > 0) and \
+            dtype in (torch.bfloat16, torch.float32):
+        done = _lib.host_ops().grouped_expert_weight_grad(
+            grads, rows, loads, max_path_load if max_path_padding else 0,
+            dtype == torch.float32, word)
+        if done is not None:
+            return done
     if not grads.is_cuda or not rows.is_cuda or not loads.is_cuda:
         raise RuntimeError("grads, rows and loads must be CUDA tensors")
     if grads.dtype != torch.bfloat16 or rows.dtype != torch.bfloat16 or \

@@ -629,6 +629,149 @@ PyObject* unsort_cells(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// ---- expert layers in 8 bits -----------------------------------------------------------------
+
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+bool matrix(const at::Tensor* t, at::ScalarType type) {
+  return t != nullptr && t->scalar_type() == type && t->dim() == 2 && t->is_contiguous() &&
+         t->numel() > 0 && t->size(1) % 16 == 0;
+}
+int64_t blocks_of(int64_t features) { return (features + 127) / 128; }
+
+// quantize_rows(rows) -> (codes, scales)
+PyObject* quantize_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    if (n != 1 || modes_active()) return nullptr;
+    const at::Tensor* x = plain(a[0]);
+    if (x == nullptr || dtype_of(*x) < 0 || !matrix(x, x->scalar_type()) || wants_grad(x) ||
+        !Place::of(*x))
+      return nullptr;
+    Memory memory;
+    const Place p(*x);
+    const int64_t L = x->size(0), width = x->size(1);
+    const int dtype = dtype_of(*x);
+    const void* const from = memory.of(x);
+    if (!aligned16(from)) return nullptr;
+    at::Tensor codes, scales;
+    int rc;
+    {
+      const Unlocked unlocked;
+      codes = empty({L, width}, at::kFloat8_e4m3fn, p.device);
+      scales = empty({blocks_of(width), L}, at::kFloat, p.device);
+      rc = brt_quantize_rows(from, codes.data_ptr(), static_cast<float*>(scales.data_ptr()), L,
+                             width, dtype, p.handle());
+      scales = scales.t();
+    }
+    if (rc != BRT_OK) return nullptr;
+    return Py_BuildValue("(NN)", THPVariable_Wrap(codes), THPVariable_Wrap(scales));
+  });
+}
+
+// grouped_expert_linear_fp8(rows, row_scales, weights, weight_scales, loads, slot, relu,
+//                           out | None, zero_unused, error_word) -> out
+PyObject* grouped_expert_linear_fp8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    if (n != 10 || modes_active()) return nullptr;
+    const at::Tensor *x = plain(a[0]), *rs = plain(a[1]), *w = plain(a[2]), *ws = plain(a[3]);
+    const at::Tensor *loads = plain(a[4]), *word = plain(a[9]), *out = nullptr;
+    if (!matrix(x, at::kFloat8_e4m3fn) || rs == nullptr || w == nullptr || ws == nullptr ||
+        loads == nullptr || word == nullptr || !Place::of(*x))
+      return nullptr;
+    const int64_t L = x->size(0), K = x->size(1);
+    if (w->scalar_type() != at::kFloat8_e4m3fn || w->dim() != 3 || !w->is_contiguous() ||
+        w->size(2) != K || w->size(1) < 1 || w->size(1) % 16 != 0)
+      return nullptr;
+    const int64_t E = w->size(0), N = w->size(1);
+    if (E < 1 || E > 1024 || rs->scalar_type() != at::kFloat || rs->dim() != 2 ||
+        rs->size(0) != L || rs->size(1) != blocks_of(K) || ws->scalar_type() != at::kFloat ||
+        ws->dim() != 3 || !ws->is_contiguous() || ws->size(0) != E ||
+        ws->size(1) != blocks_of(N) || ws->size(2) != blocks_of(K) || !int32c(loads, 1) ||
+        loads->numel() != E)
+      return nullptr;
+    for (const at::Tensor* t : {rs, w, ws, loads, word})
+      if (!same_device(*x, t)) return nullptr;
+    const long long slot = PyLong_AsLongLong(a[5]);
+    if (PyErr_Occurred()) {
+      PyErr_Clear();
+      return nullptr;
+    }
+    if (slot < 0 || slot > 0x7fffffffLL || (slot > 0 && slot * E != L)) return nullptr;
+    const int relu = truth(a[6]), zero_unused = truth(a[8]);
+    if (relu < 0 || zero_unused < 0) return nullptr;
+    if (a[7] != Py_None) {
+      out = plain(a[7]);
+      if (out == nullptr || out->scalar_type() != at::kBFloat16 || out->dim() != 2 ||
+          !out->is_contiguous() || out->size(0) != L || out->size(1) != N ||
+          !same_device(*x, out))
+        return nullptr;
+    }
+    Memory memory;
+    const Place p(*x);
+    const void *const rows = memory.of(x), *const weights = memory.of(w);
+    const auto row_scales = static_cast<const float*>(memory.of(rs));
+    const auto weight_scales = static_cast<const float*>(memory.of(ws));
+    const int32_t* const counts = memory.ints(loads);
+    void* const error = memory.of(word);
+    void* dst = memory.of(out);
+    if (!aligned16(rows) || !aligned16(weights) || !aligned16(dst)) return nullptr;
+    const int64_t row_stride = rs->stride(0), block_stride = rs->stride(1);
+    at::Tensor made;
+    int rc;
+    {
+      const Unlocked unlocked;
+      if (out == nullptr) {
+        made = empty({L, N}, at::kBFloat16, p.device);
+        dst = made.data_ptr();
+      }
+      rc = brt_grouped_expert_gemm_fp8(rows, row_scales, row_stride, block_stride, weights,
+                                       weight_scales, dst, counts, (int)E, L, (int32_t)slot, K, N,
+                                       relu, zero_unused, error, p.handle());
+    }
+    if (rc != BRT_OK) return nullptr;
+    return out != nullptr ? Py_NewRef(a[7]) : THPVariable_Wrap(made);
+  });
+}
+
+// grouped_expert_weight_grad(grads, rows, loads, slot, fp32, error_word) -> the gradients
+PyObject* grouped_expert_weight_grad(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    if (n != 6 || modes_active()) return nullptr;
+    const at::Tensor *g = plain(a[0]), *x = plain(a[1]), *loads = plain(a[2]),
+                     *word = plain(a[5]);
+    if (!matrix(g, at::kBFloat16) || !matrix(x, at::kBFloat16) || g->size(0) != x->size(0) ||
+        wants_grad(g) || wants_grad(x) || !int32c(loads, 1) || loads->numel() < 1 ||
+        loads->numel() > 1024 || word == nullptr || !Place::of(*x) || !same_device(*x, g) ||
+        !same_device(*x, loads) || !same_device(*x, word))
+      return nullptr;
+    const int64_t L = x->size(0), N = g->size(1), K = x->size(1), E = loads->numel();
+    const long long slot = PyLong_AsLongLong(a[3]);
+    if (PyErr_Occurred()) {
+      PyErr_Clear();
+      return nullptr;
+    }
+    if (slot < 0 || slot > 0x7fffffffLL || (slot > 0 && slot * E != L)) return nullptr;
+    const int wide = truth(a[4]);
+    if (wide < 0) return nullptr;
+    Memory memory;
+    const Place p(*x);
+    const void *const grads = memory.of(g), *const rows = memory.of(x);
+    const int32_t* const counts = memory.ints(loads);
+    void* const error = memory.of(word);
+    if (!aligned16(grads) || !aligned16(rows)) return nullptr;
+    at::Tensor out;
+    int rc;
+    {
+      const Unlocked unlocked;
+      out = empty({E, N, K}, wide ? at::kFloat : at::kBFloat16, p.device);
+      rc = brt_grouped_expert_weight_grad(grads, rows, out.data_ptr(), counts, (int)E, L,
+                                          (int32_t)slot, K, N, wide ? BRT_F32 : BRT_BF16, error,
+                                          p.handle());
+    }
+    if (rc != BRT_OK) return nullptr;
+    return THPVariable_Wrap(out);
+  });
+}
+
 PyMethodDef methods[] = {
     {"scan", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(scan)), METH_FASTCALL, nullptr},
     {"route_scores", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(route_scores)),
@@ -644,6 +787,14 @@ PyMethodDef methods[] = {
     {"sort_cells_fp8", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(sort_cells_fp8)),
      METH_FASTCALL, nullptr},
     {"unsort_cells", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(unsort_cells)),
+     METH_FASTCALL, nullptr},
+    {"quantize_rows", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(quantize_rows)),
+     METH_FASTCALL, nullptr},
+    {"grouped_expert_linear_fp8",
+     reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(grouped_expert_linear_fp8)),
+     METH_FASTCALL, nullptr},
+    {"grouped_expert_weight_grad",
+     reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(grouped_expert_weight_grad)),
      METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host_ops", nullptr, -1, methods,

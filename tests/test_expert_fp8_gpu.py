@@ -324,3 +324,46 @@ def test_captured_step_of_the_8_bit_layer():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, step())
+
+
+@pytest.fixture(params=["native", "python"])
+def host_side(request, monkeypatch):
+    """The operators with their native host side, and with the Python that takes what it declines."""
+    from brainstorm_b200 import _lib
+
+    if request.param == "python":
+        monkeypatch.setattr(_lib, "_host", _lib._DeclinesAll())
+    return request.param
+
+
+def test_both_host_sides(host_side):
+    from brainstorm_b200._C import expert as X
+
+    loads, N, K, slot = [3, 0, 40], 144, 272, 48
+    L = slot * len(loads)
+    x = torch.randn(L, K, device="cuda").bfloat16()
+    g = torch.randn(L, N, device="cuda").bfloat16()
+    w, ws = X.quantize_expert_weights(torch.randn(3, N, K, device="cuda"))
+    counts = torch.tensor(loads, dtype=torch.int32, device="cuda")
+    rows, rs = X.quantize_rows(x)
+    check_codes(rows, rs, x, (1,))
+    out = torch.full((L, N), 7.0, dtype=torch.bfloat16, device="cuda")
+    for _ in range(2):  # the first call makes the error word that the native side wants
+        got = X.grouped_expert_linear_fp8(rows, rs, w, ws, counts, True, slot, out=out)
+        filled = X.grouped_expert_linear_fp8(rows, rs, w, ws, counts, True, slot, True,
+                                             zero_unused=True)
+        grad = X.grouped_expert_weight_grad(g, x, counts, True, slot, torch.float32)
+        half = X.grouped_expert_weight_grad(g, x, counts, True, 0)  # the slot from the sizes
+    assert got is out and half.dtype == torch.bfloat16 and torch.equal(half, grad.bfloat16())
+    for e, load in enumerate(loads):
+        at, rest = slice(e * slot, e * slot + load), slice(e * slot + load, (e + 1) * slot)
+        a = rows[at].double() * spread(rs[at], K, 1)
+        b = w[e].double() * spread(spread(ws[e], K, 1), N, 0)
+        want, size = a @ b.t(), a.abs() @ b.abs().t()
+        tol = 140 * 2.0 ** -23 * size + 2.0 ** -8 * want.abs() + 1e-30
+        assert bool(((out[at].double() - want).abs() <= tol).all())
+        assert bool(((filled[at].double() - want.clamp(min=0)).abs() <= tol).all())
+        assert bool((out[rest] == 7).all()) and bool((filled[rest] == 0).all())
+        want = g[at].double().t() @ x[at].double()
+        size = g[at].double().abs().t() @ x[at].double().abs()
+        assert bool(((grad[e].double() - want).abs() <= (load + 2) * 2.0 ** -23 * size).all())
