@@ -280,6 +280,7 @@ class _ExpertLinearFp8(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grads):
         rows, weights, loads = ctx.saved_tensors
+        _lib.host_ops().check_capture(ctx.next_functions)
         row_grads = weight_grads = None
         if ctx.needs_input_grad[0]:
             back = quantize_expert_weights(weights, transposed=True)

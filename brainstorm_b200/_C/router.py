@@ -732,8 +732,9 @@ def order_picks(picks: torch.Tensor, path_num: int):
     twice is two rows.  Returns (places [cells, k] int32, loads [path_num] int32): path e has the
     rows from ``loads[:e].sum()`` on, in the order of the cells.  Picks outside ``[0, path_num)``
     go nowhere; their places are ``-2 - row``, naming the row at the end of the buffer that stays
-    empty.  A place may be set to -1 afterwards to leave out a pick altogether.  At most 1024
-    paths; nothing is read back to the host."""
+    empty.  (To drop picks, set them to -1 before this call: every row then is either a pick's or
+    one of the empty ones, and all of them get written.)  At most 1024 paths; nothing is read back
+    to the host."""
     done = _lib.host_ops().order_picks(picks, path_num)
     if done is not None:
         return done
@@ -821,6 +822,7 @@ class _SortCells(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, row_grads):
         (places,) = ctx.saved_tensors
+        _lib.host_ops().check_capture(ctx.next_functions)
         return _unsort(row_grads, places, None), None
 
 
@@ -836,6 +838,7 @@ class _UnsortCells(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, cell_grads):
         rows, places, gates = ctx.saved_tensors
+        _lib.host_ops().check_capture(ctx.next_functions)
         if gates is None:
             return _sort(cell_grads, places), None, None
         T, k = places.shape

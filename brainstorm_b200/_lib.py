@@ -165,6 +165,7 @@ class _DeclinesAll:
     route_scores = dispatch = combine = scan
     order_picks = sort_cells = sort_cells_fp8 = unsort_cells = scan
     quantize_rows = grouped_expert_linear_fp8 = grouped_expert_weight_grad = scan
+    check_capture = scan
 
 
 def host_ops():

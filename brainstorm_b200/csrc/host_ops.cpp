@@ -17,11 +17,14 @@
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAFunctions.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/python_cpp_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/version.h>
 
@@ -448,6 +451,27 @@ at::Tensor cells_of(const at::Tensor& rows, const at::Tensor& places, const at::
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
+// While a backward pass is captured into a CUDA graph: whether `node` hands its gradient to a leaf
+// that belongs to another stream, because an eager graph made on that stream still holds the leaf's
+// accumulator.  Autograd would then let that stream wait for the captured one, which breaks the
+// capture and may end the process.
+bool breaks_capture(torch::autograd::Node* node) {
+  if (dynamic_cast<torch::autograd::AccumulateGrad*>(node) == nullptr) return false;
+  const auto leaf_stream = node->stream();
+  return leaf_stream.has_value() &&
+         *leaf_stream != c10::cuda::getCurrentCUDAStream(leaf_stream->device_index()).unwrap();
+}
+constexpr const char* kBreaksCapture =
+    "a backward pass is being captured while an eager autograd graph of the same leaves lives on "
+    "another stream: release that graph, or capture on its stream";
+void check_capture() {
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
+  const auto node = torch::autograd::get_current_node();
+  if (node == nullptr) return;
+  for (const torch::autograd::Edge& edge : node->next_edges())
+    TORCH_CHECK(!breaks_capture(edge.function.get()), kBreaksCapture);
+}
+
 // The gradients are not differentiable themselves: asking for that says so.
 variable_list once(variable_list grads) {
   if (!c10::GradMode::is_enabled()) return grads;
@@ -467,6 +491,7 @@ struct SortCells : public torch::autograd::Function<SortCells> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list saved = ctx->get_saved_variables();
     const c10::cuda::CUDAGuard guard(saved[0].device());
+    check_capture();
     return once({cells_of(grads[0].contiguous(), saved[0], {}), at::Tensor()});
   }
 };
@@ -480,6 +505,7 @@ struct SumCells : public torch::autograd::Function<SumCells> {  // unsort withou
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list saved = ctx->get_saved_variables();
     const c10::cuda::CUDAGuard guard(saved[0].device());
+    check_capture();
     return once({sorted_rows(grads[0].contiguous(), saved[0]), at::Tensor()});
   }
 };
@@ -495,6 +521,7 @@ struct UnsortCells : public torch::autograd::Function<UnsortCells> {
     const variable_list saved = ctx->get_saved_variables();
     const at::Tensor &rows = saved[0], &places = saved[1], &gates = saved[2];
     const c10::cuda::CUDAGuard guard(places.device());
+    check_capture();
     const at::Tensor grad = grads[0].contiguous();
     const int64_t T = places.size(0), k = places.size(1);
     at::Tensor row_grads, gate_grads;
@@ -772,6 +799,24 @@ PyObject* grouped_expert_weight_grad(PyObject*, PyObject* const* a, Py_ssize_t n
   });
 }
 
+// check_capture(next_functions): the same for the node of a Python autograd function.
+PyObject* check_capture_of(PyObject*, PyObject* next) {
+  return guarded([&]() -> PyObject* {
+    if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None ||
+        !PyTuple_Check(next))
+      return nullptr;
+    for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(next); i++) {
+      PyObject* const edge = PyTuple_GET_ITEM(next, i);
+      if (!PyTuple_Check(edge) || PyTuple_GET_SIZE(edge) != 2) continue;
+      PyObject* const fn = PyTuple_GET_ITEM(edge, 0);
+      if (!torch::autograd::THPCppFunction_Check(fn)) continue;
+      auto* const node = reinterpret_cast<torch::autograd::THPCppFunction*>(fn)->cdata.get();
+      TORCH_CHECK(!breaks_capture(node), kBreaksCapture);
+    }
+    return nullptr;
+  });
+}
+
 PyMethodDef methods[] = {
     {"scan", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(scan)), METH_FASTCALL, nullptr},
     {"route_scores", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(route_scores)),
@@ -796,6 +841,7 @@ PyMethodDef methods[] = {
     {"grouped_expert_weight_grad",
      reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(grouped_expert_weight_grad)),
      METH_FASTCALL, nullptr},
+    {"check_capture", check_capture_of, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host_ops", nullptr, -1, methods,
                       nullptr, nullptr, nullptr, nullptr};

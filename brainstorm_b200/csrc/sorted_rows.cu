@@ -10,8 +10,8 @@
 //
 // A place p >= 0 is a row; p <= -2 says that the pick goes nowhere and that row -2 - p at the
 // end stays empty: sort and the row gradients write zeros there, so that every row of their
-// output is written exactly once whatever was dropped.  -1, and places outside the buffer, are
-// skipped.  Sums run in fp32 in the order of j and are rounded once; a gate of a pick that goes
+// output is written exactly once whatever was dropped.  Other numbers (-1, or outside the buffer)
+// are skipped.  Sums run in fp32 in the order of j and are rounded once; a gate of a pick that goes
 // nowhere is not looked at.
 //
 // All are bound by HBM (a few operations per byte).  sort and unsort give a warp 2 KB of a cell:

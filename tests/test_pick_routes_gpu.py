@@ -384,3 +384,45 @@ def test_an_edited_input_is_noticed_by_the_backward_pass(host_side):
     rows.mul_(2)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         out.sum().backward()
+
+
+def test_capture_beside_an_eager_graph_of_the_same_leaves_is_refused():
+    """The leaves' accumulators belong to the eager graph's stream; autograd would tie that stream to
+    the captured one.  The operator says so before, and both go on to work."""
+    from brainstorm_b200._C import expert as X
+    from brainstorm_b200._C import router as R
+
+    picks = torch.randint(0, 4, (64, 2), device="cuda")
+    places, loads = R.order_picks(picks, 4)
+    x = torch.randn(64, 32, device="cuda").bfloat16().requires_grad_()
+    gates = torch.rand(64, 2, device="cuda").requires_grad_()
+    w = (torch.randn(4, 48, 32, device="cuda") / 8).requires_grad_()
+
+    def layer():
+        y = X.expert_linear_fp8(R.sort_cells(x, places), w, loads)
+        return R.unsort_cells(y, places, gates)
+
+    steps = {
+        "sort": (lambda: R.sort_cells(x, places), (x,)),
+        "unsort": (lambda: R.unsort_cells(torch.ones(128, 32, device="cuda"), places, gates),
+                   (gates,)),
+        "layer": (layer, (w,)),
+    }
+    for name, (step, leaves) in steps.items():
+        alive = step()  # an eager graph that lives on
+        torch.autograd.grad(alive.float().sum(), leaves, retain_graph=True)
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError, match="being captured"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                out = step()
+                torch.autograd.grad(out, leaves, torch.ones_like(out))
+        torch.cuda.synchronize()
+        (want,) = torch.autograd.grad(alive.float().sum(), leaves)
+        del alive, out
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step()
+            (got,) = torch.autograd.grad(out, leaves, torch.ones_like(out))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want), name
