@@ -20,11 +20,12 @@ namespace brt_b200 {
 namespace {
 
 constexpr int kMaxPaths = 1024;
-constexpr int kWarps = 32;       // of a tile's CTA
-constexpr int kOneCtaWarps = 16;  // fewer histograms to add up
-constexpr int kBatch = 4;         // steps of 32 picks fetched together
-constexpr int kOneCta = 8192;
-constexpr int kTileMin = 2048;
+constexpr int kWarps = 32;      // of a CTA with a large tile,
+constexpr int kFewWarps = 16;   // and with few picks: fewer histograms to add up
+constexpr int kBatch = 4;       // steps of 32 picks fetched together
+// 2048 to 8192 picks took one CTA 6.4 to 20 us; two launches over tiles of 512 take 6 to 8.
+constexpr int kOneCta = 1024;
+constexpr int kSmallTile = 32 * kFewWarps;
 
 struct OrderArgs {
   const void* picks;
@@ -205,10 +206,8 @@ __global__ void __launch_bounds__(kWarps * 32) pick_place_kernel(const OrderArgs
 }
 
 int tile_for(int64_t n) {
-  const int64_t tiles = sm_count();
-  int64_t tile = (n + tiles - 1) / tiles;
-  if (tile < kTileMin) tile = kTileMin;
-  return (int)round_up((size_t)tile, kWarps * 32);
+  const int64_t tile = (n + sm_count() - 1) / sm_count();
+  return tile <= kSmallTile ? kSmallTile : (int)round_up((size_t)tile, kWarps * 32);
 }
 
 template <typename P>
@@ -230,7 +229,7 @@ int launch_order(OrderArgs a, cudaStream_t st) {
   const KernelTimer timer("pick_order", st);
   if (a.n <= kOneCta) {
     int warps = (a.n + 31) / 32;
-    if (warps > kOneCtaWarps) warps = kOneCtaWarps;
+    if (warps > kFewWarps) warps = kFewWarps;
     a.tile = (int)round_up((size_t)a.n, (size_t)warps * 32);
     const size_t smem = (size_t)(warps + 2) * buckets * sizeof(int);
     pick_order_kernel<P><<<1, warps * 32, smem, st>>>(a);
@@ -238,7 +237,8 @@ int launch_order(OrderArgs a, cudaStream_t st) {
     BRT_LAUNCH_CHECK("pick_order_kernel");
     return BRT_OK;
   }
-  pick_count_kernel<P><<<a.tiles, kWarps * 32, (size_t)kWarps * buckets * sizeof(int), st>>>(a);
+  const int warps = a.tile <= kSmallTile ? kFewWarps : kWarps;
+  pick_count_kernel<P><<<a.tiles, warps * 32, (size_t)warps * buckets * sizeof(int), st>>>(a);
   note_launch();
   BRT_LAUNCH_CHECK("pick_count_kernel");
   cudaLaunchAttribute early;
@@ -246,8 +246,8 @@ int launch_order(OrderArgs a, cudaStream_t st) {
   early.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3((unsigned)a.tiles);
-  config.blockDim = dim3(kWarps * 32);
-  config.dynamicSmemBytes = (size_t)(kWarps + 3) * buckets * sizeof(int);
+  config.blockDim = dim3((unsigned)warps * 32);
+  config.dynamicSmemBytes = (size_t)(warps + 3) * buckets * sizeof(int);
   config.stream = st;
   config.attrs = &early;
   config.numAttrs = 1;
