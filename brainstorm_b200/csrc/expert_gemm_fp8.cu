@@ -39,7 +39,9 @@
 //   warps 2-3  copy the scales of 128 rows and of the weights into a ring, one warp for each of
 //              the tile's two scale blocks, without waiting for the copies;
 //   warps 4-11 scale and accumulate, four warps for each scale block; at the end ReLU, bf16, and
-//              64 bytes of a row stored together.
+//              through shared memory out: whole groups of 32 rows by TMA stores, which go on under
+//              the next tile (with pairs; 32768 rows, 1024 -> 4096: 189 -> 175 us), an expert's
+//              last rows 64 bytes at a time.
 // Every wait is bounded: after the limit the role records an error and leaves its loop, the
 // copies in flight are given time to land, the CTAs meet, free tensor memory and return.
 #include <cuda_fp8.h>
@@ -58,22 +60,21 @@ constexpr int kBoxSizes = 4;
 constexpr int kMmaK = 32;
 // ring slots: 32 KB each with a pair, 48 KB without
 template <int kPair>
-constexpr int kStages = kPair == 2 ? 6 : 4;
+constexpr int kStages = kPair == 2 ? 5 : 4;
+// Buffers of 32 rows x 32 features in which an accumulating warp turns its rows on their way out.
+template <int kPair>
+constexpr int kOutBuffers = kPair == 2 ? 2 : 1;
+constexpr int kOutBytes = 32 * 64;
 constexpr int kScaleSlots = 4;
 constexpr int kAccWarps = 8;
 constexpr int kFirstScaleWarp = 2;
 constexpr int kFirstAccWarp = 4;  // warps are given registers by fours
 constexpr int kThreads = 32 * (kFirstAccWarp + kAccWarps);
-// The block starts with 168 registers a thread.  The accumulators alone are 128 of an
-// accumulating thread's, so the other four warps hand over what they do not need (the splits that
-// were fastest: pairs 5 to 10 % slower with the other's, single CTAs 10 %).
-template <int kPair>
-constexpr int kFewRegisters = kPair == 2 ? 88 : 56;
-template <int kPair>
-constexpr int kManyRegisters = kPair == 2 ? 208 : 224;
-static_assert(128 * kFewRegisters<1> + 32 * kAccWarps * kManyRegisters<1> == kThreads * 168 &&
-              128 * kFewRegisters<2> + 32 * kAccWarps * kManyRegisters<2> == kThreads * 168,
-              "registers");
+// The block starts with 168 registers a thread; the accumulators alone are 128 of an accumulating
+// thread's, and the other four warps hand over some of theirs (more than 184 made the compiler
+// hold more columns at once, and was up to 15 % slower).
+constexpr int kFewRegisters = 136, kManyRegisters = 184;
+static_assert(128 * kFewRegisters + 32 * kAccWarps * kManyRegisters == kThreads * 168, "registers");
 // Rows per expert on average up to which single CTAs are taken.  16 experts, 4096 -> 4096: 32 rows
 // 64 us against 80 with pairs, 128 rows 82 against 84, 256 rows 125 against 116, 1024 rows 359
 // against 319; a row in each of 64 experts, 2048 -> 4096: 97 against 139.
@@ -96,7 +97,8 @@ struct Fp8Args {
   long long N;
   int experts;
   int max_path_load;
-  int n_tiles;   // of 256 features
+  int n_tiles;         // of 256 features
+  unsigned n_inverse;  // 2^32 / n_tiles, rounded up
   int n_blocks;  // of 128 features
   int k_blocks;
   int relu;
@@ -143,11 +145,22 @@ __device__ __forceinline__ void add_scaled(float2* acc, const uint32_t (&v)[32],
                       "+f"(acc[i + 3].y));
 }
 
+// Eight accumulators as bf16, ReLU applied.
+__device__ __forceinline__ void pack_pairs(const float2* acc, int relu, uint32_t (&packed)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    float lo = acc[i].x, hi = acc[i].y;
+    if (relu) { lo = fmaxf(lo, 0.f); hi = fmaxf(hi, 0.f); }
+    const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
+    memcpy(&packed[i], &p, 4);
+  }
+}
+
 template <int kPair>
 struct alignas(1024) Fp8Smem {
   unsigned char a[kStages<kPair>][kTileBytes];               // 128 rows
   unsigned char b[kStages<kPair>][kBN / kPair * kRowBytes];  // half of a pair's features, or all
-  unsigned char turn[kAccWarps][32 * 64];
+  unsigned char out[kAccWarps][kOutBuffers<kPair>][kOutBytes];
   uint64_t full[kStages<kPair>];
   uint64_t empty[kStages<kPair>];
   uint64_t acc_full[2];
@@ -166,17 +179,42 @@ struct TileAt {
   int expert, n_tile;
   int row0, rows;  // within the expert
 };
+// Walks over the tiles of a CTA or pair, every `step`-th of all; experts are followed from the last
+// one, since a search of the whole table takes as long as two blocks of K.
 template <int kPair>
-__device__ __forceinline__ TileAt tile_at(const ExpertTable& table, const Fp8Args& g, int t) {
-  TileAt at;
-  at.expert = expert_of_tile(table, g.experts, t);
-  const int local = t - table.first_tile[at.expert];
-  const int part = local / g.n_tiles;
-  at.n_tile = local - part * g.n_tiles;
-  at.row0 = part * kPair * kBM;
-  at.rows = min(kPair * kBM, table.load[at.expert] - at.row0);
-  return at;
-}
+struct TileWalk {
+  const ExpertTable& table;
+  const Fp8Args& g;
+  int expert, local;  // number of the tile within its expert
+
+  __device__ __forceinline__ TileWalk(const ExpertTable& table_, const Fp8Args& g_, int t)
+      : table(table_), g(g_), expert(expert_of_tile(table_, g_.experts, t)),
+        local(t - table_.first_tile[expert]) {}
+  // `t`: the tile's number among all
+  __device__ __forceinline__ void to(int t, int step) {
+    local += step;
+#pragma unroll 1
+    for (int i = 0; i < 4; i++) {
+      const int tiles = table.first_tile[expert + 1] - table.first_tile[expert];
+      if (local < tiles) return;
+      local -= tiles;
+      expert++;
+    }
+    expert = expert_of_tile(table, g.experts, t);
+    local = t - table.first_tile[expert];
+  }
+  __device__ __forceinline__ TileAt at() const {
+    // local / n_tiles by its reciprocal, at most one too large
+    int part = g.n_tiles == 1 ? local : (int)__umulhi((unsigned)local, g.n_inverse);
+    if (part * g.n_tiles > local) part--;
+    TileAt at;
+    at.expert = expert;
+    at.n_tile = local - part * g.n_tiles;
+    at.row0 = part * kPair * kBM;
+    at.rows = min(kPair * kBM, table.load[expert] - at.row0);
+    return at;
+  }
+};
 // Boxes of 32 rows that CTA `rank` fetches for a tile.
 __device__ __forceinline__ int boxes_of(int rows, int rank) {
   const int mine = min(kBM, rows - rank * kBM);
@@ -202,9 +240,9 @@ __device__ __forceinline__ void zero_unused_rows(const ExpertTable& table, const
 template <int kPair>
 __global__ void __launch_bounds__(kThreads, 1)
 expert_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w,
-                       const __grid_constant__ RowMaps map_r, const Fp8Args g) {
+                       const __grid_constant__ RowMaps map_r,
+                       const __grid_constant__ CUtensorMap map_out, const Fp8Args g) {
   extern __shared__ __align__(1024) unsigned char s_raw[];
-  constexpr int kRing = kStages<kPair>;
   Fp8Smem<kPair>& s = *reinterpret_cast<Fp8Smem<kPair>*>(
       (reinterpret_cast<uintptr_t>(s_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const int warp = threadIdx.x >> 5;
@@ -220,7 +258,7 @@ expert_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w,
                         return (load + kPair * kBM - 1) / (kPair * kBM) * n_tiles;
                       });
     if (lane == 0) {
-      for (int i = 0; i < kRing; i++) {
+      for (int i = 0; i < kStages<kPair>; i++) {
         mbar_init(&s.full[i], 1);
         mbar_init(&s.empty[i], 1);
       }
@@ -242,15 +280,18 @@ expert_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w,
   tcgen05_after_sync();
   const uint32_t tmem = s.tmem_base;
   const int total_tiles = s.table.first_tile[g.experts];
+  const int first = min(group, max(total_tiles - 1, 0));
   bool failed = false;
 
   if (warp < kFirstAccWarp) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegisters<kPair>));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegisters));
     if (warp == 0) {
       int slot = 0;
       uint32_t phase = 0;
+      TileWalk<kPair> walk(s.table, g, first);
       for (int t = group; t < total_tiles && !failed; t += groups) {
-        const TileAt at = tile_at<kPair>(s.table, g, t);
+        if (t != group) walk.to(t, groups);
+        const TileAt at = walk.at();
         const int boxes = boxes_of(at.rows, rank);
         const CUtensorMap* const map_box = &map_r.box[boxes > 0 ? boxes - 1 : 0];
         const int row0 = s.table.row_base[at.expert] + at.row0 + rank * kBM;
@@ -274,7 +315,7 @@ expert_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w,
             if (boxes > 0) tma_load_2d<kPair>(s.a[slot], map_box, bar, kb * kBK, row0);
           }
           __syncwarp();
-          if (++slot == kRing) { slot = 0; phase ^= 1; }
+          if (++slot == kStages<kPair>) { slot = 0; phase ^= 1; }
         }
       }
       // copies still in flight land before the CTA's shared memory is given back
@@ -302,7 +343,7 @@ expert_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w,
               umma_commit<kPair>(&s.acc_full[buf]);
             }
             __syncwarp();
-            if (++slot == kRing) { slot = 0; phase ^= 1; }
+            if (++slot == kStages<kPair>) { slot = 0; phase ^= 1; }
             buf ^= 1;
             if (buf == 0) buf_phase ^= 1;
           }
@@ -312,8 +353,10 @@ expert_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w,
       const int half = warp - kFirstScaleWarp;
       int slot = 0;
       uint32_t phase = 0;
+      TileWalk<kPair> walk(s.table, g, first);
       for (int t = group; t < total_tiles && !failed; t += groups) {
-        const TileAt at = tile_at<kPair>(s.table, g, t);
+        if (t != group) walk.to(t, groups);
+        const TileAt at = walk.at();
         const int feature_block = min(at.n_tile * 2 + half, g.n_blocks - 1);
         const float* const ws =
             g.weight_scales + ((long long)at.expert * g.n_blocks + feature_block) * g.k_blocks;
@@ -336,19 +379,20 @@ expert_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w,
       asm volatile("cp.async.wait_all;" ::: "memory");
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegisters<kPair>));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegisters));
     const int quarter = warp & 3;  // the 32 lanes of tensor memory that this warp may read
     const int half = (warp - kFirstAccWarp) / 4;  // of the tile's features: one scale block
-    unsigned char* const turn = s.turn[warp - kFirstAccWarp];
     const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * kBM);
     const uint32_t handed_back =
         kPair == 2 ? map_to_cta(&s.acc_empty[0], 0) : smem_u32(&s.acc_empty[0]);
     const float* const row_scale = &s.row_scale[0][half][quarter * 32 + lane];
     const int row0 = rank * kBM + quarter * 32;  // of the tile
-    int buf = 0, slot = 0;
+    int buf = 0, slot = 0, out_buffer = 0;
     uint32_t buf_phase = 0, phase = 0;
+    TileWalk<kPair> walk(s.table, g, first);
     for (int t = group; t < total_tiles && !failed; t += groups) {
-      const TileAt at = tile_at<kPair>(s.table, g, t);
+      if (t != group) walk.to(t, groups);
+      const TileAt at = walk.at();
       const int feature0 = at.n_tile * kBN + half * kBM;
       const int rows = feature0 < g.N ? at.rows - row0 : 0;  // of this warp
       float2 acc[kBM / 2];
@@ -383,36 +427,52 @@ expert_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w,
         if (buf == 0) buf_phase ^= 1;
       }
       if (failed) break;
-      const int feature = feature0 + (lane & 3) * 8;
-      __nv_bfloat16* const out =
-          g.out + ((long long)s.table.row_base[at.expert] + at.row0 + row0) * g.N + feature;
+      const int row = s.table.row_base[at.expert] + at.row0 + row0;
 #pragma unroll
-      for (int c = 0; c < 4; c++) {
-        if (rows <= 0) break;
-        uint32_t packed[16];
-#pragma unroll
-        for (int i = 0; i < 16; i++) {
-          float lo = acc[c * 16 + i].x, hi = acc[c * 16 + i].y;
-          if (g.relu) { lo = fmaxf(lo, 0.f); hi = fmaxf(hi, 0.f); }
-          const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
-          memcpy(&packed[i], &p, 4);
-        }
-        // 64 bytes per row, its four pieces exchanged by the row's number: no bank conflicts
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-          *reinterpret_cast<uint4*>(turn + lane * 64 + ((i ^ (lane >> 1)) & 3) * 16) =
-              make_uint4(packed[4 * i], packed[4 * i + 1], packed[4 * i + 2], packed[4 * i + 3]);
+      for (int c = 0; c < kBM / 32; c++) {
+        const int feature = feature0 + c * 32;
+        if (rows <= 0 || feature >= g.N) break;
+        unsigned char* const staged = s.out[warp - kFirstAccWarp][out_buffer];
+        if (++out_buffer == kOutBuffers<kPair>) out_buffer = 0;  // used in turn, tile after tile
+        // the last store out of this buffer has read it (one lane issues them all)
+        if (lane == 0)
+          asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kOutBuffers<kPair> - 1)
+                       : "memory");
         __syncwarp();
+        // 64 bytes per row, its four pieces exchanged by the row's number (the 64-byte swizzle)
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-          const int row = i * 8 + (lane >> 2);
-          if (row < rows && feature + c * 32 < g.N)
-            *reinterpret_cast<uint4*>(out + (long long)row * g.N + c * 32) =
-                *reinterpret_cast<const uint4*>(turn + row * 64 + ((lane ^ (row >> 1)) & 3) * 16);
+          uint32_t packed[4];
+          pack_pairs(acc + c * 16 + i * 4, g.relu, packed);
+          *reinterpret_cast<uint4*>(staged + lane * 64 + ((i ^ (lane >> 1)) & 3) * 16) =
+              make_uint4(packed[0], packed[1], packed[2], packed[3]);
         }
-        __syncwarp();
+        if (kPair == 2 && rows >= 32) {  // the TMA stores them while the warp goes on
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) {
+            asm volatile(
+                "cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                    &map_out),
+                "r"(smem_u32(staged)), "r"(feature), "r"(row)
+                : "memory");
+          }
+        } else {  // an expert's last rows: only those that exist
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const int r = i * 8 + (lane >> 2);
+            if (r < rows && feature + (lane & 3) * 8 < g.N)
+              *reinterpret_cast<uint4*>(g.out + (long long)(row + r) * g.N + feature +
+                                        (lane & 3) * 8) =
+                  *reinterpret_cast<const uint4*>(staged + r * 64 + ((lane ^ (r >> 1)) & 3) * 16);
+          }
+          __syncwarp();
+        }
+        if (lane == 0) asm volatile("cp.async.bulk.commit_group;" ::: "memory");
       }
     }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     if (g.zero_unused)
       zero_unused_rows(s.table, g, blockIdx.x * kAccWarps + warp - kFirstAccWarp,
                        gridDim.x * kAccWarps);
@@ -427,7 +487,8 @@ expert_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w,
 }
 
 template <int kPair>
-int launch_fp8(const CUtensorMap& map_w, const RowMaps& map_r, const Fp8Args& g, cudaStream_t st) {
+int launch_fp8(const CUtensorMap& map_w, const RowMaps& map_r, const CUtensorMap& map_out,
+               const Fp8Args& g, cudaStream_t st) {
   const size_t smem = sizeof(Fp8Smem<kPair>) + 1024;
   static thread_local int configured_device = -1;
   int dev = 0;
@@ -450,7 +511,7 @@ int launch_fp8(const CUtensorMap& map_w, const RowMaps& map_r, const Fp8Args& g,
   config.attrs = &cluster;
   config.numAttrs = 1;
   const KernelTimer timer("expert_gemm_fp8_kernel", st);
-  BRT_CUDA_TRY(cudaLaunchKernelEx(&config, expert_gemm_fp8_kernel<kPair>, map_w, map_r, g));
+  BRT_CUDA_TRY(cudaLaunchKernelEx(&config, expert_gemm_fp8_kernel<kPair>, map_w, map_r, map_out, g));
   note_launch();
   return BRT_OK;
 }
@@ -526,6 +587,17 @@ BRT_API int brt_grouped_expert_gemm_fp8(const void* rows, const float* row_scale
     if (r != CUDA_SUCCESS)
       return set_error(BRT_ERR_CUDA, "cuTensorMapEncodeTiled(weights) failed with %d", (int)r);
   }
+  alignas(64) CUtensorMap map_out;
+  {
+    const cuuint64_t dims[2] = {(cuuint64_t)out_features, (cuuint64_t)total_rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)out_features * 2};
+    const cuuint32_t box[2] = {32, 32};
+    const CUresult r = encode(&map_out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, out, dims, strides, box,
+                              elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B,
+                              CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+      return set_error(BRT_ERR_CUDA, "cuTensorMapEncodeTiled(out) failed with %d", (int)r);
+  }
   Fp8Args g;
   g.loads = loads;
   g.row_scales = row_scales;
@@ -539,12 +611,14 @@ BRT_API int brt_grouped_expert_gemm_fp8(const void* rows, const float* row_scale
   g.experts = path_num;
   g.max_path_load = max_path_load;
   g.n_tiles = n_tiles;
+  g.n_inverse = n_tiles == 1 ? 0u : (unsigned)((1ULL << 32) / (unsigned)n_tiles + 1);
   g.n_blocks = n_blocks;
   g.k_blocks = (int)((in_features + kBK - 1) / kBK);
   g.relu = relu != 0;
   g.zero_unused = zero_unused != 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return pair ? launch_fp8<2>(map_w, map_r, g, st) : launch_fp8<1>(map_w, map_r, g, st);
+  return pair ? launch_fp8<2>(map_w, map_r, map_out, g, st)
+              : launch_fp8<1>(map_w, map_r, map_out, g, st);
 }
 
 }  // extern "C"
