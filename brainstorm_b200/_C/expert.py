@@ -118,9 +118,10 @@ def _loads(loads: torch.Tensor, path_num: int, dev: torch.device) -> torch.Tenso
 def quantize_rows(rows: torch.Tensor):
     """Rows [L, width] (fp32, fp16 or bf16) to 8-bit floating point with an fp32 scale for each
     128 neighbouring values: (codes [L, width] float8_e4m3fn, scales [L, ceil(width / 128)]), a
-    value is ``code * scale``.  ``scale = max(max |x|, 2**-100) / 448``.  The scales of a block lie
-    together for all rows (strides (1, L)), as the products read them.  A NaN stays NaN by itself;
-    an infinity makes its block's scale infinite.  The width must be a multiple of 16."""
+    value is ``code * scale``.  ``scale = max(max |x|, 2**-100) / 448`` and the code is the nearest to
+    ``x / scale``.  The scales of a block lie together for all rows (strides (1, L)), as the products
+    read them.  A NaN stays NaN by itself; an infinity makes its block's scale infinite and its codes
+    NaN.  The width must be a multiple of 16."""
     done = _lib.host_ops().quantize_rows(rows)
     if done is not None:
         return done

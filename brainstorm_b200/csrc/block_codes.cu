@@ -45,12 +45,13 @@ weight_codes_kernel(const typename Elem<DT>::type* __restrict__ weights,
 #pragma unroll
   for (int i = 0; i < kThreads / 32; i++) amax = fmaxf(amax, s_max[i]);
   amax = fmaxf(amax, kAmaxFloor);
+  const float scale = __fdiv_rn(amax, kCodeMax);
   const float inverse = __fdiv_rn(kCodeMax, amax);
   if (tid == 0) {
     const long long block = kTransposed
         ? (expert * gridDim.x + blockIdx.x) * gridDim.y + blockIdx.y
         : (expert * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x;
-    scales[block] = __fdiv_rn(amax, kCodeMax);
+    scales[block] = scale;
   }
   unsigned char* const out = codes + expert * N * (long long)K;
   if constexpr (!kTransposed) {
@@ -58,7 +59,7 @@ weight_codes_kernel(const typename Elem<DT>::type* __restrict__ weights,
     for (int i = 0; i < kParts; i++) {
       const int n = n0 + my_n + i;
       if (n < N && k0 + my_k < K)
-        *reinterpret_cast<uint2*>(out + (long long)n * K + k0 + my_k) = v[i].encode(inverse);
+        *reinterpret_cast<uint2*>(out + (long long)n * K + k0 + my_k) = v[i].encode(scale, inverse);
     }
   } else {
     // Row k of s_turn: the codes of 128 neighbouring n, four to a word.  A thread makes words of
@@ -68,7 +69,7 @@ weight_codes_kernel(const typename Elem<DT>::type* __restrict__ weights,
     for (int q = 0; q < kParts / 4; q++) {
       uint2 c[4];
 #pragma unroll
-      for (int i = 0; i < 4; i++) c[i] = v[q * 4 + i].encode(inverse);
+      for (int i = 0; i < 4; i++) c[i] = v[q * 4 + i].encode(scale, inverse);
 #pragma unroll
       for (int e = 0; e < 8; e++) {
         const uint32_t pick = (uint32_t)(e & 3) | (uint32_t)(4 + (e & 3)) << 4;

@@ -1,10 +1,10 @@
 // 8-bit codes (e4m3) with an fp32 scale for each block of 128 values:
-//   scale = max(max |x|, 2^-100) / 448,  code = e4m3(x * (448 / max(max |x|, 2^-100)))
-// 448 is the largest e4m3 value.  The quotients are rounded to fp32 and the product is, before the
-// rounding to a code, so a code may be the other neighbour of x / scale where that lies within
-// fp32's rounding of the middle of two codes.  The floor keeps the scale of a block of zeros, and
-// its reciprocal, finite.  NaN stays NaN and does not count for the maximum; an infinity makes
-// its block's scale infinite, and its own code NaN.
+//   scale = max(max |x|, 2^-100) / 448,  code = e4m3(x / scale)
+// 448 is the largest e4m3 value.  Both quotients are rounded to fp32 as IEEE division does: values
+// that lie in the middle of two codes are common (bf16 inputs whose maximum is a multiple of 7),
+// and a product with a rounded reciprocal sends them to either side.  The floor keeps the scale of a
+// block of zeros, and its reciprocal, finite.  NaN stays NaN and does not count for the maximum;
+// an infinity makes its block's scale infinite and its codes NaN.
 #pragma once
 
 #include <cuda_fp8.h>
@@ -70,19 +70,19 @@ struct Eight {
       return fmaxf(Elem<DT>::to_f32(m.x), Elem<DT>::to_f32(m.y));
     }
   }
-  __device__ __forceinline__ uint2 encode(float inverse) const {
-    uint32_t c[2];
+  // value / scale for all eight, from an approximate reciprocal: the remainder of the first
+  // quotient is exact, and adding its own quotient rounds correctly.
+  __device__ __forceinline__ uint2 encode(float scale, float inverse) const {
+    const float2 inv = make_float2(inverse, inverse), minus = make_float2(-scale, -scale);
+    uint32_t pair[4];
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-      const uint32_t lo = __nv_cvt_float2_to_fp8x2(
-          make_float2(value(4 * h) * inverse, value(4 * h + 1) * inverse), __NV_SATFINITE,
-          __NV_E4M3);
-      const uint32_t hi = __nv_cvt_float2_to_fp8x2(
-          make_float2(value(4 * h + 2) * inverse, value(4 * h + 3) * inverse), __NV_SATFINITE,
-          __NV_E4M3);
-      c[h] = lo | hi << 16;
+    for (int h = 0; h < 4; h++) {
+      const float2 v = make_float2(value(2 * h), value(2 * h + 1));
+      const float2 first = __fmul2_rn(v, inv);
+      const float2 rest = __ffma2_rn(first, minus, v);
+      pair[h] = __nv_cvt_float2_to_fp8x2(__ffma2_rn(rest, inv, first), __NV_SATFINITE, __NV_E4M3);
     }
-    return make_uint2(c[0], c[1]);
+    return make_uint2(pair[0] | pair[1] << 16, pair[2] | pair[3] << 16);
   }
 };
 

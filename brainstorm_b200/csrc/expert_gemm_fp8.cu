@@ -28,8 +28,8 @@
 // long as ever for however few rows, and a CTA gets twice the weights through in that time.
 //
 // What bounds it: with many rows the accumulating warps (65536 rows in 32 experts, 4096 -> 4096:
-// 1065 us, 2065 TFLOP/s; 790 us without them) and under a sustained load the 1000 W limit; with few
-// the reading of the weights (a row in each of 64 experts, 2048 -> 4096: 97 us, 5.5 TB/s).
+// 1075 us, 2046 TFLOP/s; 790 us without them) and under a sustained load the 1000 W limit; with few
+// the reading of the weights (a row in each of 64 experts, 2048 -> 4096: 100 us, 5.4 TB/s).
 // Roles inside a CTA (384 threads):
 //   warp 0     TMA loads into a shared-memory ring, 128 bytes of K per slot and row (128-byte
 //              swizzle): its 128 features, and of its 128 rows those that exist, in one box of
@@ -77,7 +77,7 @@ constexpr int kFewRegisters = 136, kManyRegisters = 184;
 static_assert(128 * kFewRegisters + 32 * kAccWarps * kManyRegisters == kThreads * 168, "registers");
 // Rows per expert on average up to which single CTAs are taken.  16 experts, 4096 -> 4096: 32 rows
 // 64 us against 80 with pairs, 128 rows 82 against 84, 256 rows 125 against 116, 1024 rows 359
-// against 319; a row in each of 64 experts, 2048 -> 4096: 97 against 139.
+// against 319; a row in each of 64 experts, 2048 -> 4096: 104 against 139.
 constexpr int kSingleRows = 192;
 constexpr uint32_t kRowBytes = kBK;
 constexpr uint32_t kTileBytes = kBM * kRowBytes;
@@ -99,7 +99,7 @@ struct Fp8Args {
   int max_path_load;
   int n_tiles;         // of 256 features
   unsigned n_inverse;  // 2^32 / n_tiles, rounded up
-  int n_blocks;  // of 128 features
+  int n_blocks;        // of 128 features
   int k_blocks;
   int relu;
   int zero_unused;

@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(kThreads) sort_codes_kernel(const SortArgs a) 
 #pragma unroll
   for (int u = 0; u < U; u++) {
     scale[u] = __shfl_sync(0xffffffffu, my_scale, (lane & 16) + u);
-    code[u] = v[u].encode(__shfl_sync(0xffffffffu, my_inverse, (lane & 16) + u));
+    code[u] = v[u].encode(scale[u], __shfl_sync(0xffffffffu, my_inverse, (lane & 16) + u));
   }
   for (int j = it.first; j < it.last; j++) {
     const int p = kPlaced ? __ldg(a.places + it.cell * a.picks + j) : 0;

@@ -418,8 +418,8 @@ BRT_API int brt_unsort_cells_backward(const void* cell_grads, const void* rows,
 
 /*
  * 8-bit floating point (e4m3) with an fp32 scale for each block of 128 values, value = code *
- * scale: scale = max(max |x|, 2^-100) / 448, code = e4m3(x * (448 / max(max |x|, 2^-100))).  No
- * counterpart in the reference.  dtype: of the values; features are multiples of 16, arrays
+ * scale: scale = max(max |x|, 2^-100) / 448, code = e4m3(x / scale), both quotients rounded to fp32.
+ * No counterpart in the reference.  dtype: of the values; features are multiples of 16, arrays
  * 16-byte aligned.
  *
  * brt_quantize_rows            rows [row_num, width] -> codes [row_num, width], scales

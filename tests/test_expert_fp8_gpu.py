@@ -367,3 +367,20 @@ def test_both_host_sides(host_side):
         want = g[at].double().t() @ x[at].double()
         size = g[at].double().abs().t() @ x[at].double().abs()
         assert bool(((grad[e].double() - want).abs() <= (load + 2) * 2.0 ** -23 * size).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_values_between_two_codes_go_to_the_even_one(dtype):
+    """bf16 and fp16 blocks whose maximum is a multiple of 7 hold many exact ties."""
+    from brainstorm_b200._C import expert as X
+
+    x = torch.arange(-140, 140, device="cuda").repeat(200)[:40 * 1280].view(40, 1280) / 128
+    x[:, ::128] = 140 / 128  # scale 5 / 2048, exact in fp32
+    x = x.to(dtype)
+    codes, scales = X.quantize_rows(x)
+    assert bool((scales == 5 / 2048).all())
+    assert torch.equal(codes.float(), (x.double() / (5 / 2048)).float()
+                       .to(torch.float8_e4m3fn).float())
+    w, _ = X.quantize_expert_weights(x[:, :1280].repeat(4, 1).view(1, 160, 1280), True)
+    want = codes.float().repeat(4, 1).view(160, 1280)
+    assert torch.equal(w[0].float().t(), want)
