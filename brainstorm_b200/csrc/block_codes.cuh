@@ -43,6 +43,8 @@ struct Eight {
   __device__ __forceinline__ float value(int i) const {
     if constexpr (DT == BRT_F32) {
       return __uint_as_float(w[i]);
+    } else if constexpr (DT == BRT_BF16) {
+      return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
     } else {
       const uint16_t bits = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
       typename Elem<DT>::type v;
