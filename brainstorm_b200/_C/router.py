@@ -732,9 +732,9 @@ def order_picks(picks: torch.Tensor, path_num: int):
     twice is two rows.  Returns (places [cells, k] int32, loads [path_num] int32): path e has the
     rows from ``loads[:e].sum()`` on, in the order of the cells.  Picks outside ``[0, path_num)``
     go nowhere; their places are ``-2 - row``, naming the row at the end of the buffer that stays
-    empty.  (To drop picks, set them to -1 before this call: every row then is either a pick's or
-    one of the empty ones, and all of them get written.)  At most 1024 paths; nothing is read back
-    to the host."""
+    empty.  (To drop picks, set them to -1 before this call.  Places may be set to -1 after it as
+    well; such a row is empty, but still one of its path's in the loads.)  At most 1024 paths;
+    nothing is read back to the host."""
     done = _lib.host_ops().order_picks(picks, path_num)
     if done is not None:
         return done
@@ -864,8 +864,9 @@ class _UnsortCells(torch.autograd.Function):
 
 def sort_cells(in_data: torch.Tensor, places: torch.Tensor) -> torch.Tensor:
     """``rows[places[t, j]] = in_data[t]``: cells [cells, ...] to [cells * k, ...] rows sorted by
-    path, ``places`` as ``order_picks`` returned them.  Rows that stay empty are zeros.  The
-    gradient of a cell is the sum of its rows' gradients (fp32, rounded once)."""
+    path, ``places`` as ``order_picks`` returned them, or with some of them set to -1 since (picks
+    that go nowhere after all).  Rows that stay empty are zeros.  The gradient of a cell is the sum
+    of its rows' gradients (fp32, rounded once)."""
     done = _lib.host_ops().sort_cells(in_data, places)
     if done is not None:
         return done

@@ -11,14 +11,26 @@
 // A place p >= 0 is a row; p <= -2 says that the pick goes nowhere and that row -2 - p at the
 // end stays empty: sort and the row gradients write zeros there, so that every row of their
 // output is written exactly once whatever was dropped.  Other numbers (-1, or outside the buffer)
-// are skipped.  Sums run in fp32 in the order of j and are rounded once; a gate of a pick that goes
-// nowhere is not looked at.
+// are skipped: places may be edited after brt_order_picks, and the rows that nothing names any more
+// are found and set to zero as well.  Sums run in fp32 in the order of j and are rounded once; a gate
+// of a pick that goes nowhere is not looked at.
 //
 // All are bound by HBM (a few operations per byte).  sort and unsort give a warp 2 KB of a cell:
 // a cell is read once for its k copies, and written once; with few cells a warp gets one pick or
 // one access per lane.  The backward of unsort
 // gives a warp one route, so that its dot product stays in the warp and is summed in one fixed
 // order; the k warps of a cell read its gradient from L1 or L2.
+//
+// Rows that no place names: a bitmap of the rows of a window, made from all places, says which of
+// them to set to zero.  Few rows are one window, and a CTA in front of the others sees to them.  For
+// more a launch of its own does, beside which the rows are moved (none of them is a row that it
+// writes): one cluster reads the places once to see whether each row is named, by their number and
+// the sums of the rows and of their squares, and only where that is not so searches the windows.
+// What that costs, bf16, places as brt_order_picks made them: 512 rows of 4 KB nothing, 8192 of 256
+// bytes 6 -> 8 us, 27003 of 128 bytes 8 -> 10 us, 65536 of 2 KB nothing (37 us), 8.4 million of 128
+// bytes 627 -> 649 us; to set all rows to zero first took those 65536 from 37 to 60 us.
+#include <cooperative_groups.h>
+
 #include "block_codes.cuh"
 
 namespace brt_b200 {
@@ -34,6 +46,16 @@ constexpr int kUnroll = VB == 16 ? 4 : 16;
 constexpr int kManyItems = 16;  // per SM
 constexpr int kManyCells = 4;   // per SM, where long items also save reads
 
+// The search for rows that no place names.
+constexpr int kFewRows = 8192;          // searched by one CTA of the kernel that moves them
+constexpr int kSearchThreads = 512;
+constexpr int kSearchCtas = 8;          // a cluster
+constexpr int kMostWindow = 40 * 8192;  // rows of a window: 40 KB of bits
+struct Unnamed {
+  int front = 0;   // CTAs in front that search
+  int beside = 0;  // a launch of its own searches, and has to end before this one does
+};
+
 struct SortArgs {
   const unsigned char* cells;
   unsigned char* rows;
@@ -47,7 +69,118 @@ struct SortArgs {
   int picks;
   int group;   // picks of an item
   int groups;  // items of a piece of a cell
+  Unnamed unnamed;
 };
+
+__device__ __forceinline__ float empty_scale() { return __fdiv_rn(kAmaxFloor, kCodeMax); }
+
+// Sets those of the rows [from, from + n) to zero that no place names, with `scales` to the codes and
+// scales of rows of zeros.  By a whole CTA; `named` has a bit for each of the rows.  (Not inlined: the loops of the
+// kernels that move rows compile as they do without it.)
+template <int VB>
+__device__ __noinline__ void clear_unnamed(unsigned* named, unsigned from, unsigned n,
+                                              const int* places, long long total,
+                                              unsigned char* rows, long long row_bytes,
+                                              float* scales) {
+  using V = typename Chunk<VB>::type;
+  const int tid = threadIdx.x, threads = blockDim.x;
+  const int words = (int)((n + 31) / 32);
+  for (int i = tid; i < words; i += threads) named[i] = 0u;
+  __syncthreads();
+  constexpr int kAtOnce = 16;
+  for (long long i0 = tid; i0 < total; i0 += (long long)threads * kAtOnce) {
+    int p[kAtOnce];
+#pragma unroll
+    for (int u = 0; u < kAtOnce; u++)
+      p[u] = i0 + (long long)u * threads < total ? __ldg(places + i0 + (long long)u * threads) : -1;
+#pragma unroll
+    for (int u = 0; u < kAtOnce; u++) {
+      const unsigned at = (unsigned)(p[u] >= 0 ? p[u] : -2 - p[u]) - from;  // -1: behind any window
+      if (at < n) atomicOr(&named[at >> 5], 1u << (at & 31));
+    }
+  }
+  __syncthreads();
+  const int lane = tid & 31;
+  for (int word = tid >> 5; word < words; word += threads >> 5) {
+    unsigned left = ~named[word];
+    if (n - word * 32u < 32u) left &= (1u << (n - word * 32u)) - 1;
+    for (; left != 0; left &= left - 1) {
+      const long long row = (long long)from + word * 32 + (__ffs(left) - 1);
+      for (long long at = lane * VB; at < row_bytes; at += 32 * VB)
+        *reinterpret_cast<V*>(rows + row * row_bytes + at) = zero_chunk<V>();
+      if (scales != nullptr)
+        for (long long b = lane; b * kCodeBlock < row_bytes; b += 32)
+          scales[b * total + row] = empty_scale();
+    }
+  }
+}
+
+// In the kernels that move rows: the CTA in front does nothing else, the last one waits for the
+// search beside (all of whose predecessors have ended, or it would not have begun).
+template <int VB>
+__device__ __forceinline__ bool searches(const Unnamed& u, const int* places, long long total,
+                                         unsigned char* rows, long long row_bytes, float* scales) {
+  __shared__ unsigned s_named[kFewRows / 32];
+  if (u.beside && blockIdx.x + 1 == gridDim.x)
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+  if ((int)blockIdx.x >= u.front) return false;
+  clear_unnamed<VB>(s_named, 0u, (unsigned)total, places, total, rows, row_bytes, scales);
+  return true;
+}
+
+struct SearchArgs {
+  const int* places;
+  unsigned char* rows;
+  float* scales;  // or null
+  long long total, row_bytes;
+  unsigned long long sum, squares;  // of 0 .. total - 1
+  unsigned window;
+};
+template <int VB>
+__global__ void __cluster_dims__(kSearchCtas) __launch_bounds__(kSearchThreads)
+unnamed_rows_kernel(const SearchArgs a) {
+  extern __shared__ unsigned s_bits[];
+  __shared__ unsigned long long s_sums[3];  // rows named, and the two sums
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const auto cluster = cooperative_groups::this_cluster();
+  const unsigned rank = cluster.block_rank();
+  if (threadIdx.x < 3) s_sums[threadIdx.x] = 0;
+  __syncthreads();
+  constexpr int kAtOnce = 16, kStep = kSearchCtas * kSearchThreads;
+  unsigned long long mine[3] = {0, 0, 0};
+  for (long long i0 = rank * kSearchThreads + threadIdx.x; i0 < a.total; i0 += kStep * kAtOnce) {
+    int p[kAtOnce];
+#pragma unroll
+    for (int u = 0; u < kAtOnce; u++)
+      p[u] = i0 + u * kStep < a.total ? __ldg(a.places + i0 + u * kStep) : -1;
+#pragma unroll
+    for (int u = 0; u < kAtOnce; u++) {
+      const unsigned row = (unsigned)(p[u] >= 0 ? p[u] : -2 - p[u]);
+      if (row >= a.total) continue;  // -1, or outside
+      mine[0]++;
+      mine[1] += row;
+      mine[2] += (unsigned long long)row * row;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 3; i++) {
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) mine[i] += __shfl_xor_sync(0xffffffffu, mine[i], d);
+    if ((threadIdx.x & 31) == 0) atomicAdd(&s_sums[i], mine[i]);
+  }
+  cluster.sync();
+  unsigned long long all[3] = {0, 0, 0};
+  for (unsigned r = 0; r < kSearchCtas; r++)
+    for (int i = 0; i < 3; i++) all[i] += cluster.map_shared_rank(s_sums, r)[i];
+  cluster.sync();  // nobody leaves while others read its sums
+  if (all[0] == (unsigned long long)a.total && all[1] == a.sum && all[2] == a.squares) return;
+  for (long long from = (long long)rank * a.window; from < a.total;
+       from += (long long)kSearchCtas * a.window) {
+    clear_unnamed<VB>(s_bits, (unsigned)from, (unsigned)min((long long)a.window, a.total - from),
+                      a.places, a.total, a.rows, a.row_bytes, a.scales);
+    __syncthreads();
+  }
+}
 
 // The item of this warp: a piece of a cell for some of its picks.
 struct SortItem {
@@ -68,8 +201,10 @@ __device__ __forceinline__ SortItem sort_item(const SortArgs& a, long long item)
 template <int VB, int U>
 __global__ void __launch_bounds__(kThreads) sort_cells_kernel(const SortArgs a) {
   using V = typename Chunk<VB>::type;
+  if (searches<VB>(a.unnamed, a.places, a.total_rows, a.rows, a.row_bytes, nullptr)) return;
   const int lane = threadIdx.x & 31;
-  const long long item = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  const long long item =
+      (long long)(blockIdx.x - a.unnamed.front) * (blockDim.x >> 5) + (threadIdx.x >> 5);
   if (item >= a.items) return;
   const SortItem it = sort_item(a, item);
   const long long at = (long long)it.piece * (32 * VB * U) + lane * VB;
@@ -99,8 +234,12 @@ constexpr int kCodeUnroll = 4;  // x 256 values per warp and item
 template <int DT, int U, bool kPlaced>
 __global__ void __launch_bounds__(kThreads) sort_codes_kernel(const SortArgs a) {
   using T = typename Elem<DT>::type;
+  if constexpr (kPlaced)
+    if (searches<16>(a.unnamed, a.places, a.total_rows, a.rows, a.width, a.scales)) return;
   const int lane = threadIdx.x & 31;
-  const long long item = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  const long long item =
+      (long long)(blockIdx.x - (kPlaced ? a.unnamed.front : 0)) * (blockDim.x >> 5) +
+      (threadIdx.x >> 5);
   if (item >= a.items) return;
   const SortItem it = sort_item(a, item);
   const long long at = (long long)it.piece * (256 * U) + lane * 8;
@@ -141,7 +280,7 @@ __global__ void __launch_bounds__(kThreads) sort_codes_kernel(const SortArgs a) 
       *reinterpret_cast<uint2*>(dst + u * 256) = p >= 0 ? code[u] : make_uint2(0u, 0u);
       if ((lane & 15) == 0)
         a.scales[((at + u * 256) / kCodeBlock) * a.total_rows + row] =
-            p >= 0 ? scale[u] : __fdiv_rn(kAmaxFloor, kCodeMax);
+            p >= 0 ? scale[u] : empty_scale();
     }
   }
 }
@@ -259,14 +398,16 @@ struct BackArgs {
   long long routes;
   long long total_rows;
   int picks;
+  Unnamed unnamed;
 };
 
 template <int DT, int VB, int kGates>
 __global__ void __launch_bounds__(kThreads) unsort_backward_kernel(const BackArgs a) {
   using V = typename Chunk<VB>::type;
   using P = Pack<DT, VB>;
+  if (searches<VB>(a.unnamed, a.places, a.total_rows, a.row_grads, a.row_bytes, nullptr)) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long route = (long long)blockIdx.x * kCtaWarps + warp;
+  const long long route = (long long)(blockIdx.x - a.unnamed.front) * kCtaWarps + warp;
   if (route >= a.routes) return;
   const int p = __ldg(a.places + route);
   const long long row = p >= 0 ? p : -2LL - p;
@@ -325,13 +466,57 @@ int access_bytes(long long row_bytes, int element, const void* a, const void* b,
       return vb;
   return element;
 }
+// The search for rows that no place names: in front of the kernel that is launched next, or beside it.
+template <int VB>
+int search_unnamed(Unnamed* u, const int* places, long long total, unsigned char* rows,
+                   long long row_bytes, float* scales, cudaStream_t st) {
+  *u = Unnamed();
+  if (total <= kFewRows) {
+    u->front = 1;
+    return BRT_OK;
+  }
+  u->beside = 1;
+  SearchArgs a;
+  a.places = places;
+  a.rows = rows;
+  a.scales = scales;
+  a.total = total;
+  a.row_bytes = row_bytes;
+  const unsigned __int128 n = (unsigned __int128)total;
+  a.sum = (unsigned long long)(n * (n - 1) / 2);
+  a.squares = (unsigned long long)(n * (n - 1) * (2 * n - 1) / 6);
+  a.window = (unsigned)round_up((size_t)((total + kSearchCtas - 1) / kSearchCtas), 32);
+  if (a.window > kMostWindow) a.window = kMostWindow;
+  unnamed_rows_kernel<VB><<<kSearchCtas, kSearchThreads, a.window / 8, st>>>(a);
+  note_launch();
+  BRT_LAUNCH_CHECK("unnamed_rows_kernel");
+  return BRT_OK;
+}
+// Launches a kernel that moves rows.
+template <typename Args>
+int launch_rows(void (*kernel)(Args), const char* name, unsigned grid, unsigned threads,
+                const Args& a, cudaStream_t st) {
+  cudaLaunchAttribute early;
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(grid);
+  config.blockDim = dim3(threads);
+  config.stream = st;
+  config.attrs = &early;
+  config.numAttrs = a.unnamed.beside;  // beside the search, else after everything before
+  BRT_CUDA_TRY(cudaLaunchKernelEx(&config, kernel, a));
+  note_launch();
+  BRT_LAUNCH_CHECK(name);
+  return BRT_OK;
+}
 // Few items: one warp per CTA spreads them over the SMs.
 struct Shape {
   unsigned grid = 0, threads = 0;
-  explicit Shape(long long items) {
+  explicit Shape(long long items, int more = 0) {
     const long long most = (long long)sm_count() * kManyItems;
     threads = items >= most ? kThreads : items * 4 >= most ? 128 : 32;
-    const long long ctas = (items + threads / 32 - 1) / (threads / 32);
+    const long long ctas = (items + threads / 32 - 1) / (threads / 32) + more;
     grid = ctas <= 0x7fffffffLL ? (unsigned)ctas : 0;
   }
 };
@@ -388,26 +573,30 @@ int launch_sort(SortArgs a, long long cells, cudaStream_t st) {
   a.group = whole ? a.picks : 1;
   a.groups = whole ? 1 : a.picks;
   a.items = cells * a.pieces * a.groups;
-  const Shape s(a.items);
-  BRT_REQUIRE(s.grid > 0, "too many cells for one launch");
   const KernelTimer timer("sort_cells_kernel", st);
-  if (whole) sort_cells_kernel<VB, kLong><<<s.grid, s.threads, 0, st>>>(a);
-  else sort_cells_kernel<VB, 1><<<s.grid, s.threads, 0, st>>>(a);
-  note_launch();
-  BRT_LAUNCH_CHECK("sort_cells_kernel");
-  return BRT_OK;
+  BRT_REQUIRE(Shape(a.items, 1).grid > 0, "too many cells for one launch");
+  const int rc = search_unnamed<VB>(&a.unnamed, a.places, a.total_rows, a.rows, a.row_bytes,
+                                    nullptr, st);
+  if (rc != BRT_OK) return rc;
+  const Shape s(a.items, a.unnamed.front);
+  return launch_rows(whole ? sort_cells_kernel<VB, kLong> : sort_cells_kernel<VB, 1>,
+                     "sort_cells_kernel", s.grid, s.threads, a, st);
 }
 
 template <int DT, int VB>
-int launch_back(const BackArgs& a, int gates, cudaStream_t st) {
-  const long long grid = (a.routes + kCtaWarps - 1) / kCtaWarps;
-  BRT_REQUIRE(grid <= 0x7fffffffLL, "too many cells for one launch");
+int launch_back(BackArgs a, int gates, cudaStream_t st) {
   const KernelTimer timer("unsort_backward_kernel", st);
-  if (gates == 1) unsort_backward_kernel<DT, VB, 1><<<(unsigned)grid, kThreads, 0, st>>>(a);
-  else unsort_backward_kernel<DT, VB, 2><<<(unsigned)grid, kThreads, 0, st>>>(a);
-  note_launch();
-  BRT_LAUNCH_CHECK("unsort_backward_kernel");
-  return BRT_OK;
+  const long long grid = (a.routes + kCtaWarps - 1) / kCtaWarps + 1;
+  BRT_REQUIRE(grid <= 0x7fffffffLL, "too many cells for one launch");
+  if (a.row_grads != nullptr) {
+    const int rc = search_unnamed<VB>(&a.unnamed, a.places, a.total_rows, a.row_grads,
+                                      a.row_bytes, nullptr, st);
+    if (rc != BRT_OK) return rc;
+  }
+  return launch_rows(gates == 1 ? unsort_backward_kernel<DT, VB, 1>
+                                : unsort_backward_kernel<DT, VB, 2>,
+                     "unsort_backward_kernel", (unsigned)grid - 1 + a.unnamed.front, kThreads, a,
+                     st);
 }
 template <int DT>
 int launch_back(const BackArgs& a, int vb, int gates, cudaStream_t st) {
@@ -426,15 +615,18 @@ int launch_codes(SortArgs a, long long cells, cudaStream_t st) {
   a.group = whole ? a.picks : 1;
   a.groups = whole ? 1 : a.picks;
   a.items = cells * a.pieces * a.groups;
-  const Shape s(a.items);
-  BRT_REQUIRE(s.grid > 0, "too many rows for one launch");
   const KernelTimer timer("sort_codes_kernel", st);
-  if (whole && threes) sort_codes_kernel<DT, 3, kPlaced><<<s.grid, s.threads, 0, st>>>(a);
-  else if (whole) sort_codes_kernel<DT, kCodeUnroll, kPlaced><<<s.grid, s.threads, 0, st>>>(a);
-  else sort_codes_kernel<DT, 1, kPlaced><<<s.grid, s.threads, 0, st>>>(a);
-  note_launch();
-  BRT_LAUNCH_CHECK("sort_codes_kernel");
-  return BRT_OK;
+  BRT_REQUIRE(Shape(a.items, 1).grid > 0, "too many rows for one launch");
+  if (kPlaced) {
+    const int rc = search_unnamed<16>(&a.unnamed, a.places, a.total_rows, a.rows, a.width,
+                                      a.scales, st);
+    if (rc != BRT_OK) return rc;
+  }
+  const Shape s(a.items, a.unnamed.front);
+  return launch_rows(whole && threes ? sort_codes_kernel<DT, 3, kPlaced>
+                     : whole         ? sort_codes_kernel<DT, kCodeUnroll, kPlaced>
+                                     : sort_codes_kernel<DT, 1, kPlaced>,
+                     "sort_codes_kernel", s.grid, s.threads, a, st);
 }
 template <bool kPlaced>
 int launch_codes(const SortArgs& a, long long cells, int dtype, cudaStream_t st) {

@@ -387,7 +387,8 @@ BRT_API int brt_order_picks(const void* picks, int picks_are_64bit, int64_t pick
 /*
  * Rows over the places [cell_num, pick_num] of brt_order_picks; a buffer of rows has
  * cell_num * pick_num of them.  Places p >= 0 are rows, p <= -2 an empty row -2 - p.  Other
- * numbers (-1, or outside the buffer) are skipped; a row that no place names is then not written.
+ * numbers (-1, or outside the buffer) are skipped; a row that no place names is empty too.  Every
+ * row of an output is written.
  *
  * brt_sort_cells      rows[places[t, j]] = cells[t], zeros in the empty rows.
  * brt_sort_cells_fp8  the same rows as brt_quantize_rows would make them; cell_size % 16 == 0,
