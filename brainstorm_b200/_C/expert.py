@@ -21,6 +21,14 @@ def _error_word(device: torch.device) -> torch.Tensor:
     return word
 
 
+def _written(out: torch.Tensor) -> torch.Tensor:
+    """``out``, a buffer of the caller's that has just been written: autograd notices when it had saved
+    what was in it."""
+    if not out.is_inference():
+        torch.autograd.graph.increment_version(out)
+    return out
+
+
 def grouped_expert_linear(rows: torch.Tensor, weights: torch.Tensor, loads: torch.Tensor,
                           max_path_padding: bool = False, max_path_load: int = 0,
                           relu: bool = False, out: torch.Tensor = None) -> torch.Tensor:
@@ -55,7 +63,8 @@ def grouped_expert_linear(rows: torch.Tensor, weights: torch.Tensor, loads: torc
         w = weights if weights.is_contiguous() else weights.contiguous()
         counts = loads if (loads.dtype == torch.int32 and loads.is_contiguous()) \
             else loads.to(torch.int32).contiguous()
-        if out is None:
+        given = out is not None
+        if not given:
             out = torch.empty((L, n_out), dtype=torch.bfloat16, device=dev)
         elif out.shape != (L, n_out) or out.dtype != torch.bfloat16 or \
                 not out.is_contiguous() or out.device != dev:
@@ -69,7 +78,7 @@ def grouped_expert_linear(rows: torch.Tensor, weights: torch.Tensor, loads: torc
             if exc.status == 4:  # BRT_ERR_UNSUPPORTED: feature counts the tiles do not divide
                 raise NotImplementedError(str(exc)) from None
             raise
-    return out
+    return _written(out) if given else out
 
 
 _DT = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
@@ -215,7 +224,8 @@ def grouped_expert_linear_fp8(rows: torch.Tensor, row_scales: torch.Tensor,
         counts = _loads(loads, E, dev)
         x, w = _aligned(rows), _aligned(weights)
         ws = weight_scales if weight_scales.is_contiguous() else weight_scales.contiguous()
-        if out is None:
+        given = out is not None
+        if not given:
             out = torch.empty((L, n_out), dtype=torch.bfloat16, device=dev)
         elif out.shape != (L, n_out) or out.dtype != torch.bfloat16 or \
                 not out.is_contiguous() or out.device != dev or out.data_ptr() % 16 != 0:
@@ -225,7 +235,7 @@ def grouped_expert_linear_fp8(rows: torch.Tensor, row_scales: torch.Tensor,
                   row_scales.stride(0), row_scales.stride(1), w.data_ptr(), ws.data_ptr(),
                   out.data_ptr(), counts.data_ptr(), E, L, slot, n_in, n_out, int(bool(relu)),
                   int(bool(zero_unused)), _error_word(dev).data_ptr(), _lib.raw_stream(dev))
-    return out
+    return _written(out) if given else out
 
 
 def grouped_expert_weight_grad(grads: torch.Tensor, rows: torch.Tensor, loads: torch.Tensor,

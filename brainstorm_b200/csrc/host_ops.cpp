@@ -755,7 +755,10 @@ PyObject* grouped_expert_linear_fp8(PyObject*, PyObject* const* a, Py_ssize_t n)
                                        relu, zero_unused, error, p.handle());
     }
     if (rc != BRT_OK) return nullptr;
-    return out != nullptr ? Py_NewRef(a[7]) : THPVariable_Wrap(made);
+    if (out == nullptr) return THPVariable_Wrap(made);
+    // autograd notices when it had saved what was in the buffer
+    if (!out->is_inference()) out->unsafeGetTensorImpl()->bump_version();
+    return Py_NewRef(a[7]);
   });
 }
 

@@ -1,0 +1,67 @@
+"""Calls of the expert layers that write buffers which autograd has saved."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(params=["native", "python"])
+def host_side(request, monkeypatch):
+    from brainstorm_b200 import _lib
+
+    if request.param == "python":
+        monkeypatch.setattr(_lib, "_host", _lib._DeclinesAll())
+    return request.param
+
+
+def layer(L=96, N=128, K=128, E=3, seed=0):
+    """Operands of one expert layer in 8 bits and in bf16, 32 rows each but for the last expert."""
+    from brainstorm_b200._C import expert as X
+
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn(L, K, device="cuda", generator=gen).bfloat16()
+    w = (torch.randn(E, N, K, device="cuda", generator=gen) / 8).bfloat16()
+    loads = torch.full((E,), L // E, dtype=torch.int32, device="cuda")
+    return X.quantize_rows(x) + X.quantize_expert_weights(w), (x, w), loads
+
+
+def products():
+    from brainstorm_b200._C import expert as X
+
+    fp8, bf16, loads = layer()
+    return {
+        "fp8": lambda **kw: X.grouped_expert_linear_fp8(*fp8, loads, **kw),
+        "bf16": lambda **kw: X.grouped_expert_linear(*bf16, loads, **kw),
+    }
+
+
+# ------------------------------------------------------------------------------ buffers of the caller
+@pytest.mark.parametrize("kind", ["fp8", "bf16"])
+def test_a_saved_buffer_that_is_written_again_is_noticed(host_side, kind):
+    """One buffer for the rows of two micro-batches: the first one's backward pass must not take the
+    second one's rows."""
+    from brainstorm_b200._C import router as R
+
+    product = products()[kind]
+    picks = torch.arange(96, device="cuda").view(48, 2) % 3
+    places, _ = R.order_picks(picks, 3)
+    gates = torch.rand(48, 2, device="cuda", requires_grad=True)
+    buf = torch.empty(96, 128, dtype=torch.bfloat16, device="cuda")
+    for _ in range(2):  # the first call makes what the native side wants
+        before = buf._version
+        assert product(out=buf) is buf and buf._version == before + 1
+    out = R.unsort_cells(buf, places, gates)
+    product(out=buf)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.float().sum().backward()
+
+
+@pytest.mark.parametrize("kind", ["fp8", "bf16"])
+def test_buffers_made_in_inference_mode(host_side, kind):
+    product = products()[kind]
+    want = product()
+    with torch.inference_mode():
+        buf = torch.empty_like(want)
+        assert torch.equal(product(out=buf), want)
+        buf.zero_()
+    assert torch.equal(product(out=buf), want)
