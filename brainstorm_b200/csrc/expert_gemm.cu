@@ -274,10 +274,9 @@ expert_gemm_kernel(const __grid_constant__ CUtensorMap map_w,
         buffer ^= 1;
 #pragma unroll
         for (int i = 0; i < 16; i++) {
-          float lo = __uint_as_float(v[2 * i]);
-          float hi = __uint_as_float(v[2 * i + 1]);
-          if (g.relu) { lo = fmaxf(lo, 0.f); hi = fmaxf(hi, 0.f); }
-          const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
+          __nv_bfloat162 p = __floats2bfloat162_rn(__uint_as_float(v[2 * i]),
+                                                   __uint_as_float(v[2 * i + 1]));
+          if (g.relu) p = relu_pair(p);
           turn[(2 * i) * 32 + lane] = p.x;
           turn[(2 * i + 1) * 32 + lane] = p.y;
         }

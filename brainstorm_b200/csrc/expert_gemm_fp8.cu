@@ -149,10 +149,9 @@ __device__ __forceinline__ void add_scaled(float2* acc, const uint32_t (&v)[32],
 __device__ __forceinline__ void pack_pairs(const float2* acc, int relu, uint32_t (&packed)[4]) {
 #pragma unroll
   for (int i = 0; i < 4; i++) {
-    float lo = acc[i].x, hi = acc[i].y;
-    if (relu) { lo = fmaxf(lo, 0.f); hi = fmaxf(hi, 0.f); }
-    const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
-    memcpy(&packed[i], &p, 4);
+    const __nv_bfloat162 p = __floats2bfloat162_rn(acc[i].x, acc[i].y);
+    const __nv_bfloat162 q = relu ? relu_pair(p) : p;
+    memcpy(&packed[i], &q, 4);
   }
 }
 

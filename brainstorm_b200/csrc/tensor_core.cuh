@@ -234,6 +234,10 @@ __device__ __forceinline__ void tmem_free(uint32_t base) {
                  "r"(kTmemCols)
                  : "memory");
 }
+// ReLU that keeps NaN: a maximum that ignores it would turn a row gone wrong into zeros.
+__device__ __forceinline__ __nv_bfloat162 relu_pair(__nv_bfloat162 p) {
+  return __hmax2_nan(p, __nv_bfloat162(__float2bfloat16_rn(0.f), __float2bfloat16_rn(0.f)));
+}
 __device__ __forceinline__ void tcgen05_before_sync() {
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
 }

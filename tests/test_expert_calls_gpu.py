@@ -1,4 +1,5 @@
-"""Calls of the expert layers that write buffers which autograd has saved."""
+"""Calls of the expert layers that touch more than their numbers: buffers that autograd has saved, NaN
+under a fused ReLU."""
 import pytest
 import torch
 
@@ -65,3 +66,55 @@ def test_buffers_made_in_inference_mode(host_side, kind):
         assert torch.equal(product(out=buf), want)
         buf.zero_()
     assert torch.equal(product(out=buf), want)
+
+
+# ------------------------------------------------------------------------------------------- ReLU
+@pytest.mark.parametrize("rows_per_expert", [5, 40, 300])
+def test_relu_keeps_nan_8_bit(host_side, rows_per_expert):
+    """NaN in a row, in a weight and in a scale, and infinities of both signs that meet: what
+    torch.relu makes of the product without it."""
+    from brainstorm_b200._C import expert as X
+
+    E, N, K = 3, 272, 272
+    L = E * rows_per_expert
+    torch.manual_seed(1)
+    xq, xs = X.quantize_rows(torch.randn(L, K, device="cuda"))
+    wq, ws = X.quantize_expert_weights(torch.randn(E, N, K, device="cuda"))
+    nan = torch.tensor(float("nan"), device="cuda").to(torch.float8_e4m3fn)
+    xq[3, 200] = nan
+    wq[1, 17, 5] = nan
+    xs = xs.clone()
+    xs[rows_per_expert * 2 + 1, 0] = float("nan")
+    xs[4, 0], xs[4, 1] = float("inf"), float("-inf")
+    loads = torch.full((E,), rows_per_expert, dtype=torch.int32, device="cuda")
+    for _ in range(2):
+        plain = X.grouped_expert_linear_fp8(xq, xs, wq, ws, loads)
+        got = X.grouped_expert_linear_fp8(xq, xs, wq, ws, loads, relu=True)
+    X.check_status()
+    assert bool(plain[3].isnan().all()) and bool(plain[rows_per_expert:, 17][:5].isnan().all())
+    assert bool(plain[rows_per_expert * 2 + 1].isnan().all()) and bool(plain[4].isnan().any())
+    assert torch.equal(got.isnan(), plain.isnan())
+    assert torch.equal(got.nan_to_num(), torch.relu(plain).nan_to_num())
+    assert bool((plain.nan_to_num() < 0).any())
+
+
+@pytest.mark.parametrize("rows_per_expert", [5, 40, 300])
+@pytest.mark.parametrize("N", [128, 256])
+def test_relu_keeps_nan_bf16(rows_per_expert, N):
+    from brainstorm_b200._C import expert as X
+
+    E, K = 3, 128
+    L = E * rows_per_expert
+    torch.manual_seed(2)
+    x = torch.randn(L, K, device="cuda").bfloat16()
+    w = torch.randn(E, N, K, device="cuda").bfloat16()
+    x[3, 100] = float("nan")
+    w[1, 17, 5] = float("nan")
+    x[4, 0], x[4, 1] = float("inf"), float("inf")  # weights of both signs: inf - inf
+    loads = torch.full((E,), rows_per_expert, dtype=torch.int32, device="cuda")
+    plain = X.grouped_expert_linear(x, w, loads)
+    got = X.grouped_expert_linear(x, w, loads, relu=True)
+    X.check_status()
+    assert bool(plain[3].isnan().all()) and bool(plain[4].isnan().any())
+    assert torch.equal(got.isnan(), plain.isnan())
+    assert torch.equal(got.nan_to_num(), torch.relu(plain).nan_to_num())
