@@ -193,7 +193,8 @@ def grouped_expert_linear_fp8(rows: torch.Tensor, row_scales: torch.Tensor,
     ``weight_scales`` [E, ceil(out / 128), ceil(in / 128)] fp32.  The scales may be any fp32
     numbers; sums run in fp32.  Returns [L, out] bf16.  Rows beyond an expert's load are left
     unwritten, or set to zero with ``zero_unused``.  ``in`` and ``out`` are multiples of 16.  The
-    other arguments are those of ``grouped_expert_linear``."""
+    other arguments are those of ``grouped_expert_linear``.  No gradient: train through
+    ``expert_linear_fp8``."""
     word = _error_words.get(rows.get_device())
     if word is not None and (not max_path_padding or max_path_load > 0):
         done = _lib.host_ops().grouped_expert_linear_fp8(
@@ -216,6 +217,8 @@ def grouped_expert_linear_fp8(rows: torch.Tensor, row_scales: torch.Tensor,
             weight_scales.shape != (E, _blocks(n_out), _blocks(n_in)):
         raise RuntimeError("expected fp32 row_scales [L, in / 128] and weight_scales "
                            "[E, out / 128, in / 128], rounded up")
+    _no_gradient("grouped_expert_linear_fp8", rows, row_scales, weights, weight_scales,
+                 *(() if out is None else (out,)))
     dev = rows.device
     if any(t.device != dev for t in (row_scales, weights, weight_scales)):
         raise RuntimeError("rows, weights and their scales are on different devices")

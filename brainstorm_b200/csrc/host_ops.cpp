@@ -702,7 +702,8 @@ PyObject* grouped_expert_linear_fp8(PyObject*, PyObject* const* a, Py_ssize_t n)
     const at::Tensor *x = plain(a[0]), *rs = plain(a[1]), *w = plain(a[2]), *ws = plain(a[3]);
     const at::Tensor *loads = plain(a[4]), *word = plain(a[9]), *out = nullptr;
     if (!matrix(x, at::kFloat8_e4m3fn) || rs == nullptr || w == nullptr || ws == nullptr ||
-        loads == nullptr || word == nullptr || !Place::of(*x))
+        loads == nullptr || word == nullptr || wants_grad(x) || wants_grad(rs) || wants_grad(w) ||
+        wants_grad(ws) || !Place::of(*x))
       return nullptr;
     const int64_t L = x->size(0), K = x->size(1);
     if (w->scalar_type() != at::kFloat8_e4m3fn || w->dim() != 3 || !w->is_contiguous() ||
@@ -728,7 +729,7 @@ PyObject* grouped_expert_linear_fp8(PyObject*, PyObject* const* a, Py_ssize_t n)
     if (a[7] != Py_None) {
       out = plain(a[7]);
       if (out == nullptr || out->scalar_type() != at::kBFloat16 || out->dim() != 2 ||
-          !out->is_contiguous() || out->size(0) != L || out->size(1) != N ||
+          !out->is_contiguous() || out->size(0) != L || out->size(1) != N || wants_grad(out) ||
           !same_device(*x, out))
         return nullptr;
     }

@@ -1,5 +1,5 @@
 """Calls of the expert layers that touch more than their numbers: buffers that autograd has saved, NaN
-under a fused ReLU."""
+under a fused ReLU, operands that want gradients."""
 import pytest
 import torch
 
@@ -118,3 +118,34 @@ def test_relu_keeps_nan_bf16(rows_per_expert, N):
     assert bool(plain[3].isnan().all()) and bool(plain[4].isnan().any())
     assert torch.equal(got.isnan(), plain.isnan())
     assert torch.equal(got.nan_to_num(), torch.relu(plain).nan_to_num())
+
+
+# ------------------------------------------------------------------------------------ derivatives
+@pytest.mark.parametrize("which", range(4))
+def test_the_8_bit_product_refuses_operands_that_want_gradients(host_side, which):
+    from brainstorm_b200._C import expert as X
+
+    fp8, _, loads = layer()
+    want = X.grouped_expert_linear_fp8(*fp8, loads)
+    leaf = fp8[which].float().requires_grad_()
+    operands = list(fp8)
+    operands[which] = leaf.to(fp8[which].dtype)  # still part of the leaf's graph
+    for _ in range(2):
+        with pytest.raises(RuntimeError, match="no gradient"):
+            X.grouped_expert_linear_fp8(*operands, loads)
+    with torch.no_grad():
+        assert torch.equal(X.grouped_expert_linear_fp8(*operands, loads), want)
+
+
+def test_the_8_bit_product_refuses_a_buffer_that_wants_a_gradient(host_side):
+    from brainstorm_b200._C import expert as X
+
+    fp8, _, loads = layer()
+    want = X.grouped_expert_linear_fp8(*fp8, loads)
+    buf = torch.zeros_like(want).requires_grad_()
+    with pytest.raises(RuntimeError, match="no gradient"):
+        X.grouped_expert_linear_fp8(*fp8, loads, out=buf)
+    assert bool((buf == 0).all())
+    with torch.no_grad():
+        assert X.grouped_expert_linear_fp8(*fp8, loads, out=buf) is buf
+    assert torch.equal(buf.detach(), want)
