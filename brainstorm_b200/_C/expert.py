@@ -105,6 +105,7 @@ def _check_features(*features: int) -> None:
 def _no_gradient(name: str, *tensors: torch.Tensor) -> None:
     if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
         raise RuntimeError(f"{name} has no gradient: use expert_linear_fp8, or no_grad()")
+    _lib.refuse_tangents(name, *tensors)
 
 
 def _slot(max_path_padding: bool, max_path_load: int, total_rows: int, path_num: int) -> int:
@@ -320,6 +321,7 @@ def expert_linear_fp8(rows: torch.Tensor, weights: torch.Tensor, loads: torch.Te
         raise NotImplementedError("expert_linear_fp8 takes bf16 rows and bf16 or fp32 weights")
     if rows.dim() != 2 or weights.dim() != 3 or weights.size(2) != rows.size(1):
         raise RuntimeError("expected rows [L, in] and weights [E, out, in]")
+    _lib.refuse_tangents("expert_linear_fp8", rows, weights)
     return _ExpertLinearFp8.apply(rows, weights, loads, bool(max_path_padding),
                                   int(max_path_load))
 

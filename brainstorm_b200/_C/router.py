@@ -823,6 +823,7 @@ class _SortCells(torch.autograd.Function):
     def backward(ctx, row_grads):
         (places,) = ctx.saved_tensors
         _lib.host_ops().check_capture(ctx.next_functions)
+        _lib.refuse_tangents("the gradient of sort_cells", row_grads)
         return _unsort(row_grads, places, None), None
 
 
@@ -839,6 +840,7 @@ class _UnsortCells(torch.autograd.Function):
     def backward(ctx, cell_grads):
         rows, places, gates = ctx.saved_tensors
         _lib.host_ops().check_capture(ctx.next_functions)
+        _lib.refuse_tangents("the gradient of unsort_cells", cell_grads)
         if gates is None:
             return _sort(cell_grads, places), None, None
         T, k = places.shape
@@ -873,6 +875,7 @@ def sort_cells(in_data: torch.Tensor, places: torch.Tensor) -> torch.Tensor:
     places = _check_places(places, in_data, "in_data")
     if in_data.size(0) != places.size(0):
         raise RuntimeError(f"{in_data.size(0)} cells but places of {places.size(0)}")
+    _lib.refuse_tangents("sort_cells", in_data)
     if in_data.requires_grad and torch.is_grad_enabled():
         return _SortCells.apply(in_data, places)
     return _sort(in_data, places)
@@ -891,6 +894,7 @@ def sort_cells_fp8(in_data: torch.Tensor, places: torch.Tensor):
                            f"{tuple(in_data.shape)}")
     if in_data.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("sort_cells_fp8 has no gradient: use sort_cells, or no_grad()")
+    _lib.refuse_tangents("sort_cells_fp8", in_data)
     T, k = places.shape
     width = in_data.size(1)
     if width < 1 or width % 16 != 0:
@@ -923,6 +927,7 @@ def unsort_cells(rows: torch.Tensor, places: torch.Tensor,
             raise RuntimeError("gates must have the shape and device of places")
         if gates.dtype not in (torch.float32, rows.dtype):
             raise RuntimeError("gates must be float32 or match the data type")
+    _lib.refuse_tangents("unsort_cells", rows, gates)
     if torch.is_grad_enabled() and (rows.requires_grad or
                                     (gates is not None and gates.requires_grad)):
         return _UnsortCells.apply(rows, places, gates)

@@ -168,6 +168,16 @@ class _DeclinesAll:
     check_capture = scan
 
 
+def refuse_tangents(name: str, *tensors) -> None:
+    """For an operator without a forward-mode derivative: a tensor that carries one does not require
+    a gradient, and its derivative would vanish without a word."""
+    from torch.autograd import forward_ad
+
+    if forward_ad._current_level >= 0 and any(
+            forward_ad.unpack_dual(t).tangent is not None for t in tensors if t is not None):
+        raise RuntimeError(f"{name} has no forward-mode derivative")
+
+
 def host_ops():
     """The native host side of the hot operators (``csrc/host_ops.cpp``).  It is built against one
     torch; where it is missing or belongs to another one, a warning says so (once) and the Python

@@ -34,7 +34,8 @@ namespace {
 
 PyObject* g_dense;  // attribute name on index tensors
 
-// A plain torch.Tensor (no subclass, no functional wrapper) with memory on the GPU.
+// A plain torch.Tensor (no subclass, no functional wrapper) with memory on the GPU and without a
+// forward-mode derivative.
 const at::Tensor* plain(PyObject* o) {
   if (!THPVariable_CheckExact(o)) return nullptr;
   const at::Tensor& t = THPVariable_Unpack(o);
@@ -43,6 +44,7 @@ const at::Tensor* plain(PyObject* o) {
           c10::DispatchKeySet({c10::DispatchKey::Python, c10::DispatchKey::Functionalize,
                                c10::DispatchKey::Negative, c10::DispatchKey::Conjugate})))
     return nullptr;
+  if (t._fw_grad(0).defined()) return nullptr;
   return &t;
 }
 bool modes_active() {
@@ -472,6 +474,11 @@ void check_capture() {
     TORCH_CHECK(!breaks_capture(edge.function.get()), kBreaksCapture);
 }
 
+// Neither have the gradients forward-mode derivatives.
+void refuse_tangent(const at::Tensor& grad) {
+  TORCH_CHECK(!grad._fw_grad(0).defined(),
+              "the gradients of sorted rows have no forward-mode derivative");
+}
 // The gradients are not differentiable themselves: asking for that says so.
 variable_list once(variable_list grads) {
   if (!c10::GradMode::is_enabled()) return grads;
@@ -492,6 +499,7 @@ struct SortCells : public torch::autograd::Function<SortCells> {
     const variable_list saved = ctx->get_saved_variables();
     const c10::cuda::CUDAGuard guard(saved[0].device());
     check_capture();
+    refuse_tangent(grads[0]);
     return once({cells_of(grads[0].contiguous(), saved[0], {}), at::Tensor()});
   }
 };
@@ -506,6 +514,7 @@ struct SumCells : public torch::autograd::Function<SumCells> {  // unsort withou
     const variable_list saved = ctx->get_saved_variables();
     const c10::cuda::CUDAGuard guard(saved[0].device());
     check_capture();
+    refuse_tangent(grads[0]);
     return once({sorted_rows(grads[0].contiguous(), saved[0]), at::Tensor()});
   }
 };
@@ -522,6 +531,7 @@ struct UnsortCells : public torch::autograd::Function<UnsortCells> {
     const at::Tensor &rows = saved[0], &places = saved[1], &gates = saved[2];
     const c10::cuda::CUDAGuard guard(places.device());
     check_capture();
+    refuse_tangent(grads[0]);
     const at::Tensor grad = grads[0].contiguous();
     const int64_t T = places.size(0), k = places.size(1);
     at::Tensor row_grads, gate_grads;

@@ -1,5 +1,6 @@
-"""Calls of the expert layers that touch more than their numbers: buffers that autograd has saved, NaN
-under a fused ReLU, operands that want gradients."""
+"""Calls of the expert layers and of the routes by picks that touch more than their numbers: buffers that
+autograd has saved, NaN under a fused ReLU, operands that want gradients or carry forward-mode
+derivatives."""
 import pytest
 import torch
 
@@ -149,3 +150,70 @@ def test_the_8_bit_product_refuses_a_buffer_that_wants_a_gradient(host_side):
     with torch.no_grad():
         assert X.grouped_expert_linear_fp8(*fp8, loads, out=buf) is buf
     assert torch.equal(buf.detach(), want)
+
+
+FORWARD = ["sort_cells", "sort_cells_fp8", "unsort_cells", "unsort_cells gates", "quantize_rows",
+           "quantize_expert_weights", "linear rows' scales", "linear weights' scales", "weight_grad",
+           "weight_grad rows", "expert_linear_fp8", "expert_linear_fp8 weights"]
+
+
+@pytest.mark.parametrize("wants_grad", [False, True])
+@pytest.mark.parametrize("name", FORWARD)
+def test_forward_mode_derivatives_are_refused(host_side, name, wants_grad):
+    """They would vanish without a word: no operator here has a forward-mode derivative."""
+    import torch.autograd.forward_ad as fw
+
+    from brainstorm_b200._C import expert as X
+    from brainstorm_b200._C import router as R
+
+    fp8, (x, w), loads = layer()
+    X.grouped_expert_linear_fp8(*fp8, loads)
+    places, _ = R.order_picks(torch.arange(96, device="cuda").view(48, 2) % 3, 3)
+    cells, gates = x[:48].contiguous(), torch.rand(48, 2, device="cuda")
+    grads = torch.randn(96, 128, device="cuda").bfloat16()
+    calls = {
+        "sort_cells": (cells, lambda t: R.sort_cells(t, places)),
+        "sort_cells_fp8": (cells, lambda t: R.sort_cells_fp8(t, places)),
+        "unsort_cells": (x, lambda t: R.unsort_cells(t, places)),
+        "unsort_cells gates": (gates, lambda t: R.unsort_cells(x, places, t)),
+        "quantize_rows": (x, X.quantize_rows),
+        "quantize_expert_weights": (w, X.quantize_expert_weights),
+        "linear rows' scales": (
+            fp8[1], lambda t: X.grouped_expert_linear_fp8(fp8[0], t, *fp8[2:], loads)),
+        "linear weights' scales": (
+            fp8[3], lambda t: X.grouped_expert_linear_fp8(*fp8[:3], t, loads)),
+        "weight_grad": (grads, lambda t: X.grouped_expert_weight_grad(t, x, loads)),
+        "weight_grad rows": (x, lambda t: X.grouped_expert_weight_grad(grads, t, loads)),
+        "expert_linear_fp8": (x, lambda t: X.expert_linear_fp8(t, w, loads)),
+        "expert_linear_fp8 weights": (w, lambda t: X.expert_linear_fp8(x, t, loads)),
+    }
+    value, call = calls[name]
+    call(value)
+    value = value.detach().clone().requires_grad_(wants_grad)
+    with fw.dual_level():
+        dual = fw.make_dual(value, torch.ones_like(value))
+        with pytest.raises((RuntimeError, NotImplementedError), match="forward|no gradient|jvp"):
+            call(dual)
+        call(value.detach())  # without a tangent all is as ever
+
+
+@pytest.mark.parametrize("name", ["sort_cells", "unsort_cells", "unsort_cells gates", "layer"])
+def test_forward_mode_derivatives_of_gradients_are_refused(host_side, name):
+    import torch.autograd.forward_ad as fw
+
+    from brainstorm_b200._C import expert as X
+    from brainstorm_b200._C import router as R
+
+    _, (x, w), loads = layer()
+    places, _ = R.order_picks(torch.arange(96, device="cuda").view(48, 2) % 3, 3)
+    leaf = (x[:48] if name == "sort_cells" else x).detach().clone().requires_grad_()
+    gates = torch.rand(48, 2, device="cuda") if name.endswith("gates") else None
+    out = {"sort_cells": lambda: R.sort_cells(leaf, places),
+           "layer": lambda: X.expert_linear_fp8(leaf, w, loads)}.get(
+               name, lambda: R.unsort_cells(leaf, places, gates))()
+    gy = torch.randn_like(out)
+    with fw.dual_level():
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch.autograd.grad(out, leaf, fw.make_dual(gy, torch.ones_like(gy)),
+                                retain_graph=True)
+        torch.autograd.grad(out, leaf, gy)
