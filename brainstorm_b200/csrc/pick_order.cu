@@ -210,6 +210,13 @@ int tile_for(int64_t n) {
   return tile <= kSmallTile ? kSmallTile : (int)round_up((size_t)tile, kWarps * 32);
 }
 
+// A tile ends at most 1024 picks per SM behind the last pick, which is within 32 bits; pick_total +
+// tile is not.
+int tiles_for(int64_t n) {
+  const int64_t tile = tile_for(n);
+  return (int)((n + tile - 1) / tile);
+}
+
 template <typename P>
 int launch_order(OrderArgs a, cudaStream_t st) {
   const int buckets = a.paths + 1;
@@ -266,8 +273,7 @@ extern "C" {
 
 BRT_API size_t brt_pick_order_scratch_bytes(int64_t pick_total, int path_num) {
   if (pick_total <= kOneCta || path_num <= 0) return 0;
-  const int64_t tile = tile_for(pick_total);
-  return (size_t)((pick_total + tile - 1) / tile) * (size_t)(path_num + 1) * sizeof(int);
+  return (size_t)tiles_for(pick_total) * (size_t)(path_num + 1) * sizeof(int);
 }
 
 BRT_API int brt_order_picks(const void* picks, int picks_are_64bit, int64_t pick_total,
@@ -297,7 +303,7 @@ BRT_API int brt_order_picks(const void* picks, int picks_are_64bit, int64_t pick
   a.n = (int)pick_total;
   a.paths = path_num;
   a.tile = tile_for(pick_total);
-  a.tiles = (a.n + a.tile - 1) / a.tile;
+  a.tiles = tiles_for(pick_total);
   return picks_are_64bit ? launch_order<long long>(a, st) : launch_order<int>(a, st);
 }
 
