@@ -262,7 +262,7 @@ expert_gemm_kernel(const __grid_constant__ CUtensorMap map_w,
       __nv_bfloat16* const out =
           g.out + first_row * g.N + (long long)(at.m_tile * kPair + (int)rank) * kBM +
           quarter * 32 + my_piece;
-      if (!mbar_wait(&s.acc_full[acc], acc_phase)) { failed = true; break; }
+      if (!mbar_wait_warp(&s.acc_full[acc], acc_phase)) { failed = true; break; }
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
       for (int c0 = 0; c0 < rows; c0 += 32) {

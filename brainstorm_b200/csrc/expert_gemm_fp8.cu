@@ -301,7 +301,7 @@ expert_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w,
                 kRowBytes +
             (uint32_t)blocks * kTileBytes;
         for (int kb = 0; kb < g.k_blocks; kb++) {
-          if (!mbar_wait(&s.empty[slot], phase ^ 1)) { failed = true; break; }
+          if (!mbar_wait_warp(&s.empty[slot], phase ^ 1)) { failed = true; break; }
           if (elect_one()) {
             if (rank == 0) mbar_expect_tx(&s.full[slot], bytes);  // of both CTAs
             const uint32_t bar =
@@ -326,7 +326,8 @@ expert_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w,
         uint32_t phase = 0, buf_phase = 0;
         for (int t = group; t < total_tiles && !failed; t += groups) {
           for (int kb = 0; kb < g.k_blocks; kb++) {
-            if (!mbar_wait(&s.acc_empty[buf], buf_phase ^ 1) || !mbar_wait(&s.full[slot], phase)) {
+            if (!mbar_wait_warp(&s.acc_empty[buf], buf_phase ^ 1) ||
+                !mbar_wait_warp(&s.full[slot], phase)) {
               failed = true;
               break;
             }
@@ -364,7 +365,7 @@ expert_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w,
             ((long long)s.table.row_base[at.expert] + at.row0 + row0) * g.row_stride;
 #pragma unroll 1
         for (int kb = 0; kb < g.k_blocks; kb++) {
-          if (!mbar_wait(&s.scale_empty[slot][half], phase ^ 1)) { failed = true; break; }
+          if (!mbar_wait_warp(&s.scale_empty[slot][half], phase ^ 1)) { failed = true; break; }
 #pragma unroll
           for (int i = 0; i < kBM / 32; i++)
             if (row0 + i * 32 < at.rows)
@@ -399,9 +400,9 @@ expert_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w,
       for (int i = 0; i < kBM / 2; i++) acc[i] = make_float2(0.f, 0.f);
 #pragma unroll 1
       for (int kb = 0; kb < g.k_blocks; kb++) {
-        if (!mbar_wait(&s.scale_full[slot][half], phase)) { failed = true; break; }
+        if (!mbar_wait_warp(&s.scale_full[slot][half], phase)) { failed = true; break; }
         const float scale = row_scale[slot * 2 * kBM] * s.weight_scale[slot][half];
-        if (!mbar_wait(&s.acc_full[buf], buf_phase)) { failed = true; break; }
+        if (!mbar_wait_warp(&s.acc_full[buf], buf_phase)) { failed = true; break; }
         tcgen05_after_sync();
         const uint32_t from = lanes + (uint32_t)(buf * kBN);
         uint32_t v[2][32];

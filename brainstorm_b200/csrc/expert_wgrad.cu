@@ -208,7 +208,7 @@ expert_wgrad_kernel(const __grid_constant__ CUtensorMap map_g,
         const int n0 = at.n0 + (int)rank * kBM;
         const int k0 = at.k0 + (int)rank * half;
         for (int i = 0; i < at.blocks; i++) {
-          if (!mbar_wait(&s.empty[slot], phase ^ 1)) { failed = true; break; }
+          if (!mbar_wait_warp(&s.empty[slot], phase ^ 1)) { failed = true; break; }
           if (elect_one()) {
             uint32_t bar;
             if (at.load - i * kBR < kBR) {  // the expert ends here: warp 2 passes the slot on
@@ -245,8 +245,8 @@ expert_wgrad_kernel(const __grid_constant__ CUtensorMap map_g,
          t = wgrad_turn(++round, group, groups)) {
           const WgradTile at = wgrad_tile<kPair>(s, g, t);
           for (int i = 0; i < at.blocks; i++) {
-            if ((i % kChunk == 0 && !mbar_wait(&s.acc_empty[acc], acc_phase ^ 1)) ||
-                !mbar_wait(&s.full[slot], phase)) {
+            if ((i % kChunk == 0 && !mbar_wait_warp(&s.acc_empty[acc], acc_phase ^ 1)) ||
+                !mbar_wait_warp(&s.full[slot], phase)) {
               failed = true;
               break;
             }
@@ -280,7 +280,7 @@ expert_wgrad_kernel(const __grid_constant__ CUtensorMap map_g,
         const int rows = at.load % kBR;
         if (rows != 0) {
           const int last = (slot + at.blocks - 1) % kRing;
-          if (!mbar_wait(&s.tail[last], (phases >> last) & 1)) { failed = true; break; }
+          if (!mbar_wait_warp(&s.tail[last], (phases >> last) & 1)) { failed = true; break; }
           phases ^= 1u << last;
           const int until = (rows + kMmaK - 1) / kMmaK * kMmaK;
           const int pieces = (until - rows) * 8;  // of 16 bytes, in one box
@@ -318,7 +318,7 @@ expert_wgrad_kernel(const __grid_constant__ CUtensorMap map_g,
       for (int i = 0; i < kBN / 2; i++) sum[i] = 0.f;
 #pragma unroll 1
       for (int i = 0; i < at.blocks; i += kChunk) {
-        if (!mbar_wait(&s.acc_full[acc], acc_phase)) { failed = true; break; }
+        if (!mbar_wait_warp(&s.acc_full[acc], acc_phase)) { failed = true; break; }
         tcgen05_after_sync();
 #pragma unroll
         for (int c = 0; c < 4; c++) {

@@ -45,26 +45,47 @@ __device__ __forceinline__ bool elect_one() {
       : "=r"(yes));
   return yes != 0;
 }
-// Bounded wait for the phase with the given parity; false when the limit ran out.
+__device__ __forceinline__ bool mbar_try_wait(uint32_t addr, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+      "selp.u32 %0, 1, 0, p;\n"
+      "}\n"
+      : "=r"(done)
+      : "r"(addr), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+// Bounded wait for the phase with the given parity, by one lane; false when the limit ran out.
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity) {
   const uint32_t addr = smem_u32(bar);
   unsigned long long until = 0;
   for (int spin = 0;; spin++) {
-    uint32_t done;
-    asm volatile(
-        "{\n"
-        ".reg .pred p;\n"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
-        "selp.u32 %0, 1, 0, p;\n"
-        "}\n"
-        : "=r"(done)
-        : "r"(addr), "r"(parity)
-        : "memory");
-    if (done) return true;
+    if (mbar_try_wait(addr, parity)) return true;
     if (spin > 64) {
       const unsigned long long now = now_ns();
       if (until == 0) until = now + kWaitLimitNs;
       else if (now > until) return false;
+      __nanosleep(32);
+    }
+  }
+}
+// The same by a whole warp, whose lanes go on together or give up together: were that left to each
+// lane, those that give up while the phase completes would miss the warp-wide instructions behind the
+// wait, and the others would wait for them there without a limit.
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity,
+                                               unsigned long long limit_ns = kWaitLimitNs) {
+  const uint32_t addr = smem_u32(bar);
+  unsigned long long until = 0;
+  for (int spin = 0;; spin++) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(addr, parity))) return true;
+    if (spin > 64) {
+      const unsigned long long now = now_ns();
+      const bool late = until != 0 && now > until;
+      if (until == 0) until = now + limit_ns;
+      if (__any_sync(0xffffffffu, late)) return false;
       __nanosleep(32);
     }
   }

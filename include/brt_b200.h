@@ -415,6 +415,14 @@ BRT_API int brt_unsort_cells_backward(const void* cell_grads, const void* rows,
                                       int64_t cell_size, int dtype, int gates_dtype,
                                       void* stream);
 
+/*
+ * For tests of the bounded waits inside the expert products: one warp waits for a barrier on which
+ * another arrives after `arrive_after_ns`; lane 0 gives up after `first_limit_ns`, the others after
+ * `limit_ns` (each at most 1e8).  results[32]: whether the lane saw the barrier complete.
+ */
+BRT_API int brt_expert_wait_probe(int32_t* results, uint64_t first_limit_ns, uint64_t limit_ns,
+                                  uint64_t arrive_after_ns, void* stream);
+
 /* ------------------------------------------------------------------ experts: 8-bit products */
 
 /*
