@@ -413,12 +413,8 @@ expert_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w,
           if (c < 3) {
             tmem_load_32(from + (c + 1) * 32, v[(c + 1) & 1]);
           } else {  // everything is in registers: the next block may be multiplied into it
-            tcgen05_before_sync();
-            __syncwarp();
-            if (lane == 0) {
-              mbar_arrive_cluster_relaxed(handed_back + buf * (uint32_t)sizeof(uint64_t));
-              mbar_arrive(&s.scale_empty[slot][half]);
-            }
+            hand_back(handed_back + buf * (uint32_t)sizeof(uint64_t));
+            if (lane == 0) mbar_arrive(&s.scale_empty[slot][half]);
           }
           add_scaled(acc + c * 16, v[c & 1], scale);
         }

@@ -328,12 +328,7 @@ expert_wgrad_kernel(const __grid_constant__ CUtensorMap map_g,
           tmem_load_wait();
           add_columns(sum + c * 32, v);
         }
-        tcgen05_before_sync();
-        __syncwarp();
-        if (lane == 0) {
-          if (rank == 0) mbar_arrive(&s.acc_empty[acc]);
-          else mbar_arrive_cluster_relaxed(map_to_cta(&s.acc_empty[acc], 0));
-        }
+        hand_back(kPair == 2 ? map_to_cta(&s.acc_empty[acc], 0) : smem_u32(&s.acc_empty[acc]));
         if (++acc == 2) { acc = 0; acc_phase ^= 1; }
       }
       if (failed) break;
