@@ -16,7 +16,13 @@ _error_words = {}
 def _error_word(device: torch.device) -> torch.Tensor:
     word = _error_words.get(device.index)
     if word is None:
-        word = torch.zeros(1, dtype=torch.int32, device=device)
+        word = torch.empty(1, dtype=torch.int32, device=device)
+        if torch.cuda.is_current_stream_capturing():
+            # not by the graph, whose replays would set it to zero again
+            with torch.cuda.stream(torch.cuda.Stream(device)):
+                word.zero_()
+        else:
+            word.zero_()
         _error_words[device.index] = word
     return word
 

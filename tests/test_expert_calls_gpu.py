@@ -1,6 +1,6 @@
-"""Calls of the expert layers and of the routes by picks that touch more than their numbers: buffers that
-autograd has saved, NaN under a fused ReLU, operands that want gradients or carry forward-mode
-derivatives."""
+"""Calls of the expert layers that touch more than their numbers: buffers that autograd has saved, NaN
+under a fused ReLU, operands that want gradients or carry forward-mode derivatives, first calls under
+capture."""
 import pytest
 import torch
 
@@ -217,3 +217,30 @@ def test_forward_mode_derivatives_of_gradients_are_refused(host_side, name):
             torch.autograd.grad(out, leaf, fw.make_dual(gy, torch.ones_like(gy)),
                                 retain_graph=True)
         torch.autograd.grad(out, leaf, gy)
+
+
+# ---------------------------------------------------------------------------------------- capture
+def test_a_report_survives_the_replays_of_a_graph_captured_before_any_eager_call(monkeypatch):
+    """The word that reports a wait which ran out is made by the first call.  When that call is
+    captured, replays must not wipe out what a kernel reported in between."""
+    from brainstorm_b200 import _lib
+    from brainstorm_b200._C import expert as X
+
+    fp8, _, loads = layer()
+    want = X.grouped_expert_linear_fp8(*fp8, loads)
+    torch.cuda.synchronize()
+    monkeypatch.setattr(X, "_error_words", {})
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = X.grouped_expert_linear_fp8(*fp8, loads)
+    torch.cuda.synchronize()
+    X.check_status()  # zero before the graph has run once
+    graph.replay()
+    X.check_status()
+    assert torch.equal(out, want)
+    (word,) = X._error_words.values()
+    word.fill_(7)
+    graph.replay()
+    with pytest.raises(_lib.BrtError):
+        X.check_status()
+    X.check_status()
