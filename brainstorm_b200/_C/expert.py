@@ -115,9 +115,9 @@ def _no_gradient(name: str, *tensors: torch.Tensor) -> None:
 
 
 def _slot(max_path_padding: bool, max_path_load: int, total_rows: int, path_num: int) -> int:
-    if not max_path_padding:
+    if not max_path_padding or total_rows == 0:
         return 0
-    slot = int(max_path_load) if max_path_load > 0 else total_rows // path_num
+    slot = int(max_path_load) if max_path_load > 0 else total_rows // max(path_num, 1)
     if slot * path_num != total_rows or slot < 1:
         raise RuntimeError("a padded buffer must hold max_path_load rows per expert")
     return slot

@@ -244,3 +244,83 @@ def test_a_report_survives_the_replays_of_a_graph_captured_before_any_eager_call
     with pytest.raises(_lib.BrtError):
         X.check_status()
     X.check_status()
+
+
+# ------------------------------------------------------------------------------------- empty batches
+@pytest.mark.parametrize("padded", [False, True])
+def test_a_batch_without_rows(host_side, padded):
+    """Serving and training of no cells at all: empty results, weights' gradients of zeros."""
+    from brainstorm_b200._C import expert as X
+    from brainstorm_b200._C import router as R
+
+    E, N, K = 3, 128, 256
+    picks = torch.empty(0, 2, dtype=torch.int64, device="cuda")
+    cells = torch.empty(0, K, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    gates = torch.empty(0, 2, device="cuda", requires_grad=True)
+    w = torch.randn(E, N, K, device="cuda", requires_grad=True)
+    places, loads = R.order_picks(picks, E)
+    with torch.no_grad():
+        wq, ws = X.quantize_expert_weights(w)
+        for _ in range(2):
+            codes, scales = R.sort_cells_fp8(cells, places)
+            y = X.grouped_expert_linear_fp8(codes, scales, wq, ws, loads, padded)
+            assert y.shape == (0, N) and R.unsort_cells(y, places, gates).shape == (0, N)
+            grad = X.grouped_expert_weight_grad(y, R.sort_cells(cells, places), loads, padded)
+            assert grad.shape == (E, N, K) and bool((grad == 0).all())
+    y = X.expert_linear_fp8(R.sort_cells(cells, places), w, loads, padded)
+    out = R.unsort_cells(y, places, gates)
+    grads = torch.autograd.grad(out, (cells, gates, w), torch.empty_like(out))
+    assert grads[0].shape == (0, K) and grads[1].shape == (0, 2)
+    assert bool((grads[2] == 0).all())
+    X.check_status()
+
+
+def test_no_experts_are_refused(host_side):
+    from brainstorm_b200._C import expert as X
+
+    rows = torch.randn(8, 32, device="cuda").bfloat16()
+    codes, scales = X.quantize_rows(rows)
+    wq, ws = X.quantize_expert_weights(torch.empty(0, 32, 32, device="cuda"))
+    loads = torch.empty(0, dtype=torch.int32, device="cuda")
+    for padded in (False, True):
+        with pytest.raises(RuntimeError):
+            X.grouped_expert_linear_fp8(codes, scales, wq, ws, loads, padded)
+        with pytest.raises(RuntimeError):
+            X.grouped_expert_weight_grad(rows, rows, loads, padded)
+
+
+# ----------------------------------------------------------------------------------- calls at once
+def test_layers_on_two_streams_at_once():
+    """Everything that a layer launches, on two streams with inputs of their own, again and again."""
+    from brainstorm_b200._C import expert as X
+    from brainstorm_b200._C import router as R
+
+    T, k, E, d, n = 6000, 2, 12, 256, 384
+    made = []
+    for seed in (1, 2):
+        gen = torch.Generator(device="cuda").manual_seed(seed)
+        made.append((torch.randint(-1, E, (T, k), device="cuda", generator=gen),
+                     torch.randn(T, d, device="cuda", generator=gen).bfloat16(),
+                     torch.randn(E, n, d, device="cuda", generator=gen).bfloat16(),
+                     torch.rand(T, k, device="cuda", generator=gen),
+                     torch.randn(T, n, device="cuda", generator=gen).bfloat16()))
+
+    def step(picks, x, w, gates, gy):
+        x, w, gates = (t.detach().requires_grad_() for t in (x, w, gates))
+        places, loads = R.order_picks(picks, E)
+        out = R.unsort_cells(X.expert_linear_fp8(R.sort_cells(x, places), w, loads), places, gates)
+        return (out.detach(),) + torch.autograd.grad(out, (x, w, gates), gy)
+
+    want = [step(*m) for m in made]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(8):
+        for i in (0, 1):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(step(*made[i]))
+    torch.cuda.synchronize()
+    X.check_status()
+    for i in (0, 1):
+        for outs in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(outs, want[i]))
