@@ -198,10 +198,10 @@ def grouped_expert_linear_fp8(rows: torch.Tensor, row_scales: torch.Tensor,
     ``rows`` [L, in] float8_e4m3fn with ``row_scales`` [L, ceil(in / 128)] fp32 (any strides), as
     ``sort_cells_fp8`` or ``quantize_rows`` return them; ``weights`` [E, out, in] float8_e4m3fn with
     ``weight_scales`` [E, ceil(out / 128), ceil(in / 128)] fp32.  The scales may be any fp32
-    numbers; sums run in fp32.  Returns [L, out] bf16.  Rows beyond an expert's load are left
-    unwritten, or set to zero with ``zero_unused``.  ``in`` and ``out`` are multiples of 16.  The
-    other arguments are those of ``grouped_expert_linear``.  No gradient: train through
-    ``expert_linear_fp8``."""
+    numbers whose products are in fp32's normal range; sums run in fp32.  Returns [L, out] bf16.
+    Rows beyond an expert's load are left unwritten, or set to zero with ``zero_unused``.  ``in``
+    and ``out`` are multiples of 16.  The other arguments are those of ``grouped_expert_linear``.
+    No gradient: train through ``expert_linear_fp8``."""
     word = _error_words.get(rows.get_device())
     if word is not None and (not max_path_padding or max_path_load > 0):
         done = _lib.host_ops().grouped_expert_linear_fp8(

@@ -2,9 +2,11 @@
 //   scale = max(max |x|, 2^-100) / 448,  code = e4m3(x / scale)
 // 448 is the largest e4m3 value.  Both quotients are rounded to fp32 as IEEE division does: values
 // that lie in the middle of two codes are common (bf16 inputs whose maximum is a multiple of 7),
-// and a product with a rounded reciprocal sends them to either side.  The floor keeps the scale of a
-// block of zeros, and its reciprocal, finite.  NaN stays NaN and does not count for the maximum;
-// an infinity makes its block's scale infinite and its codes NaN.
+// and a product with a rounded reciprocal sends them to either side.  Where max / 448 itself is
+// rounded, a value in the middle of two codes by the unrounded quotient may lie 2^-24 beside it and
+// goes to that side: 8 in 10000 codes of bf16 values then are the other one of two codes equally near.
+// The floor keeps the scale of a block of zeros, and its reciprocal, finite.  NaN stays NaN and does
+// not count for the maximum; an infinity makes its block's scale infinite and its codes NaN.
 #pragma once
 
 #include <cuda_fp8.h>
@@ -72,8 +74,9 @@ struct Eight {
       return fmaxf(Elem<DT>::to_f32(m.x), Elem<DT>::to_f32(m.y));
     }
   }
-  // value / scale for all eight, from an approximate reciprocal: the remainder of the first
-  // quotient is exact, and adding its own quotient rounds correctly.
+  // value / scale for all eight, from an approximate reciprocal, by Markstein's last step of a
+  // division: the remainder of the first quotient is exact, and adding its own quotient rounds
+  // correctly.
   __device__ __forceinline__ uint2 encode(float scale, float inverse) const {
     const float2 inv = make_float2(inverse, inverse), minus = make_float2(-scale, -scale);
     uint32_t pair[4];

@@ -27,9 +27,10 @@
 // each) for many rows, single CTAs (128 x 256) for few: there the work on a block of K takes as
 // long as ever for however few rows, and a CTA gets twice the weights through in that time.
 //
-// What bounds it: with many rows the accumulating warps (65536 rows in 32 experts, 4096 -> 4096:
-// 1075 us, 2046 TFLOP/s; 790 us without them) and under a sustained load the 1000 W limit; with few
-// the reading of the weights (a row in each of 64 experts, 2048 -> 4096: 100 us, 5.4 TB/s).
+// What bounds it: with many rows the accumulating warps (65536 rows in 32 even experts, 4096 -> 4096,
+// three calls in a row: 1077 us, 2043 TFLOP/s; 790 us without them) and under a sustained load the
+// 1000 W limit (uneven experts, for seconds: 1290 to 1330 us, 1650 to 1700 TFLOP/s); with few the
+// reading of the weights (a row in each of 64 experts, 2048 -> 4096, calls in a row: 100 us, 5.4 TB/s).
 // Roles inside a CTA (384 threads):
 //   warp 0     TMA loads into a shared-memory ring, 128 bytes of K per slot and row (128-byte
 //              swizzle): its 128 features, and of its 128 rows those that exist, in one box of
@@ -72,12 +73,16 @@ constexpr int kFirstAccWarp = 4;  // warps are given registers by fours
 constexpr int kThreads = 32 * (kFirstAccWarp + kAccWarps);
 // The block starts with 168 registers a thread; the accumulators alone are 128 of an accumulating
 // thread's, and the other four warps hand over some of theirs (more than 184 made the compiler
-// hold more columns at once, and was up to 15 % slower).
+// hold more columns at once, and was up to 15 % slower).  At 168, ptxas -v counts 16 bytes of spill
+// stores and 64 of spill loads per thread, in both forms.
 constexpr int kFewRegisters = 136, kManyRegisters = 184;
 static_assert(128 * kFewRegisters + 32 * kAccWarps * kManyRegisters == kThreads * 168, "registers");
-// Rows per expert on average up to which single CTAs are taken.  16 experts, 4096 -> 4096: 32 rows
-// 64 us against 80 with pairs, 128 rows 82 against 84, 256 rows 125 against 116, 1024 rows 359
-// against 319; a row in each of 64 experts, 2048 -> 4096: 104 against 139.
+// Rows per expert on average up to which single CTAs are taken.  16 experts, 4096 -> 4096, 16 calls
+// in a row: 32 rows 58 us against 81 with pairs, 128 rows 64 against 87, 194 rows 102 against 93,
+// 256 rows 105 against 95, 1024 rows 328 against 289; a row in each of 64 experts, 2048 -> 4096: 100
+// against 146.
+// The loads are on the device, so rows that dropped picks leave empty count here, and padded slots
+// count as full: slots of more than 192 rows with few of them used take the slower form.
 constexpr int kSingleRows = 192;
 constexpr uint32_t kRowBytes = kBK;
 constexpr uint32_t kTileBytes = kBM * kRowBytes;

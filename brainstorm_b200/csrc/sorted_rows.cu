@@ -75,13 +75,14 @@ struct SortArgs {
 __device__ __forceinline__ float empty_scale() { return __fdiv_rn(kAmaxFloor, kCodeMax); }
 
 // Sets those of the rows [from, from + n) to zero that no place names, with `scales` to the codes and
-// scales of rows of zeros.  By a whole CTA; `named` has a bit for each of the rows.  (Not inlined: the loops of the
-// kernels that move rows compile as they do without it.)
+// scales of rows of zeros.  By a whole CTA; `named` has a bit for each of the rows.  Not inlined: the
+// loops of the kernels that move rows compile as they do without it (inlined, the backward pass of
+// unsort went from 215 to 185 us over 131072 rows of 4 KB and from 178 to 239 over 120000 of 2002 bytes).
 template <int VB>
 __device__ __noinline__ void clear_unnamed(unsigned* named, unsigned from, unsigned n,
-                                              const int* places, long long total,
-                                              unsigned char* rows, long long row_bytes,
-                                              float* scales) {
+                                           const int* places, long long total,
+                                           unsigned char* rows, long long row_bytes,
+                                           float* scales) {
   using V = typename Chunk<VB>::type;
   const int tid = threadIdx.x, threads = blockDim.x;
   const int words = (int)((n + 31) / 32);

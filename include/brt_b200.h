@@ -449,8 +449,9 @@ BRT_API int brt_quantize_expert_weights(const void* weights, void* codes, float*
  * brt_grouped_expert_gemm over such codes:
  *   out[r, n] = act(sum over b of row_scales[r, b] * weight_scales[e, n / 128, b]
  *                   * sum over k in block b of rows[r, k] * weights[e, n, k])
- * with fp32 sums and bf16 out.  row_scales: element (r, b) at r * scale_row_stride + b *
- * scale_block_stride.  Everything else as there; in_features % 16 == 0 and out_features % 16 == 0.
+ * with fp32 sums and bf16 out.  The product of the two scales is rounded to fp32 before it meets the
+ * sum: below 2^-126 it loses digits, from 2^128 on it is infinite.  row_scales: element (r, b) at
+ * r * scale_row_stride + b * scale_block_stride.  Everything else as there; in_features % 16 == 0 and out_features % 16 == 0.
  * zero_unused != 0 writes zeros to the rows of `out` that belong to no expert.
  */
 BRT_API int brt_grouped_expert_gemm_fp8(const void* rows, const float* row_scales,
