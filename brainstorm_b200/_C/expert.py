@@ -6,6 +6,8 @@ src/backend/torch/jit.cc:54-75; benchmark/switch_moe/switch_expert.py:62-99 buil
 a Switch layer from them).  This op consumes the same buffer and the same per-expert loads,
 with the loads staying on the device.
 """
+import ctypes
+
 import torch
 
 from .. import _lib
@@ -13,16 +15,23 @@ from .. import _lib
 _error_words = {}
 
 
+class _Word:
+    """An int32 at an address on the device, as ``torch.as_tensor`` takes it without a copy."""
+
+    def __init__(self, address: int):
+        self.__cuda_array_interface__ = {"shape": (1,), "typestr": "<i4", "data": (address, False),
+                                         "version": 2}
+
+
 def _error_word(device: torch.device) -> torch.Tensor:
     word = _error_words.get(device.index)
     if word is None:
-        word = torch.empty(1, dtype=torch.int32, device=device)
-        if torch.cuda.is_current_stream_capturing():
-            # not by the graph, whose replays would set it to zero again
-            with torch.cuda.stream(torch.cuda.Stream(device)):
-                word.zero_()
-        else:
-            word.zero_()
+        # the library's own memory: what is allocated while a graph is captured belongs to the graph,
+        # whose replays write to it
+        at = ctypes.c_void_p()
+        with _lib.device_guard(device):
+            _lib.call("brt_expert_error_word", ctypes.byref(at))
+            word = torch.as_tensor(_Word(at.value), device=device)
         _error_words[device.index] = word
     return word
 

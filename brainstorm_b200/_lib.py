@@ -61,6 +61,7 @@ SIGNATURES = {
     "brt_sum_rows_by_index": (_int, [_vp, _vp, _vp, _i64, _i64, _i64, _int, _vp, _sz, _vp]),
     "brt_grouped_expert_gemm": (_int, [_vp, _vp, _vp, _vp, _int, _i64, _i32, _i64, _i64, _int,
                                        _vp, _vp]),
+    "brt_expert_error_word": (_int, [_vp]),
     "brt_expert_wait_probe": (_int, [_vp, _u64, _u64, _u64, _vp]),
     "brt_pick_order_scratch_bytes": (_sz, [_i64, _int]),
     "brt_order_picks": (_int, [_vp, _int, _i64, _int, _vp, _vp, _vp, _sz, _vp]),

@@ -79,9 +79,19 @@ int sm_count() {
   return cached;
 }
 
+__device__ int g_expert_error_word;  // zero when the library is loaded
+
 }  // namespace brt_b200
 
 extern "C" {
+
+BRT_API int brt_expert_error_word(void** word) {
+  using namespace brt_b200;
+  clear_error();
+  BRT_REQUIRE(word != nullptr, "word is null");
+  BRT_CUDA_TRY(cudaGetSymbolAddress(word, g_expert_error_word));
+  return BRT_OK;
+}
 
 BRT_API int brt_abi_version(void) { return 3; }
 

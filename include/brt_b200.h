@@ -416,6 +416,12 @@ BRT_API int brt_unsort_cells_backward(const void* cell_grads, const void* rows,
                                       void* stream);
 
 /*
+ * *word: the address of an int of the library's on the current device, zero until a kernel that was
+ * given it as its error_word reports.  May be called while a stream is being captured.
+ */
+BRT_API int brt_expert_error_word(void** word);
+
+/*
  * For tests of the bounded waits inside the expert products: one warp waits for a barrier on which
  * another arrives after `arrive_after_ns`; lane 0 gives up after `first_limit_ns`, the others after
  * `limit_ns` (each at most 1e8).  results[32]: whether the lane saw the barrier complete.

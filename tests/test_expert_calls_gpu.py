@@ -246,6 +246,52 @@ def test_a_report_survives_the_replays_of_a_graph_captured_before_any_eager_call
     X.check_status()
 
 
+def test_a_report_is_not_written_by_what_else_a_graph_computes(monkeypatch):
+    """Nor may the word share memory with what the capture that made it has let go."""
+    from brainstorm_b200._C import expert as X
+
+    fp8, _, loads = layer()
+    want = X.grouped_expert_linear_fp8(*fp8, loads)
+    torch.cuda.synchronize()
+    monkeypatch.setattr(X, "_error_words", {})
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for n in (1, 100, 1000, 100000):
+            gone = torch.full((n,), 5, dtype=torch.int32, device="cuda")
+            del gone
+        out = X.grouped_expert_linear_fp8(*fp8, loads)
+    for _ in range(2):
+        graph.replay()
+        X.check_status()
+    assert torch.equal(out, want)
+
+
+def test_the_first_product_of_a_process_may_be_captured():
+    """Then even the library's kernels and its word are loaded under capture."""
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    code = """
+import torch
+from brainstorm_b200._C import expert as X
+rows, scales = torch.randn(96, 128, device="cuda").to(torch.float8_e4m3fn), torch.ones(96, 1, device="cuda")
+w, ws = torch.randn(3, 128, 128, device="cuda").to(torch.float8_e4m3fn), torch.ones(3, 1, 1, device="cuda")
+loads = torch.full((3,), 32, dtype=torch.int32, device="cuda")
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out = X.grouped_expert_linear_fp8(rows, scales, w, ws, loads)
+graph.replay()
+X.check_status()
+assert torch.equal(out, X.grouped_expert_linear_fp8(rows, scales, w, ws, loads))
+print("fine")
+"""
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300,
+                          cwd=Path(__file__).resolve().parent.parent)
+    assert done.returncode == 0 and "fine" in done.stdout, done.stderr[-2000:]
+
+
 # ------------------------------------------------------------------------------------- empty batches
 @pytest.mark.parametrize("padded", [False, True])
 def test_a_batch_without_rows(host_side, padded):

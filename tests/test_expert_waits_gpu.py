@@ -29,3 +29,10 @@ def test_lanes_go_on_together_or_not_at_all(first, others, arrives, done):
         _lib.call("brt_expert_wait_probe", results.data_ptr(), first, others, arrives,
                   torch.cuda.current_stream().cuda_stream)
         assert results.tolist() == [done] * 32
+
+
+def test_the_word_of_run_out_waits_needs_a_place():
+    from brainstorm_b200 import _lib
+
+    with pytest.raises(_lib.BrtError, match="null"):
+        _lib.call("brt_expert_error_word", None)
