@@ -24,11 +24,13 @@
 // Rows that no place names: a bitmap of the rows of a window, made from all places, says which of
 // them to set to zero.  Few rows are one window, and a CTA in front of the others sees to them.  For
 // more a launch of its own does, beside which the rows are moved (none of them is a row that it
-// writes): one cluster reads the places once to see whether each row is named, by their number and
-// the sums of the rows and of their squares, and only where that is not so searches the windows.
+// writes): one cluster reads the places once to see whether each row is named, and only where that is
+// not so searches the windows.  It goes by the number of rows named and by a sum of 64-bit mixtures of
+// them (the finisher of splitmix64), which other rows than 0, 1, .. share by an accident of 2^-64.
 // What that costs, bf16, places as brt_order_picks made them: 512 rows of 4 KB nothing, 8192 of 256
-// bytes 6 -> 8 us, 27003 of 128 bytes 8 -> 10 us, 65536 of 2 KB nothing (37 us), 8.4 million of 128
-// bytes 627 -> 649 us; to set all rows to zero first took those 65536 from 37 to 60 us.
+// bytes 8 us as before, 27003 of 128 bytes 8 -> 11 us, 65536 of 2 KB nothing (37 us), 524288 of 64
+// bytes 45 -> 52 us, 8.4 million of 128 bytes 627 -> 670 us; to set all rows to zero first took those
+// 65536 from 37 to 60 us.
 #include <cooperative_groups.h>
 
 #include "block_codes.cuh"
@@ -134,21 +136,26 @@ struct SearchArgs {
   unsigned char* rows;
   float* scales;  // or null
   long long total, row_bytes;
-  unsigned long long sum, squares;  // of 0 .. total - 1
   unsigned window;
 };
+__device__ __forceinline__ unsigned long long mixed(unsigned row) {
+  unsigned long long x = (row + 1ull) * 0x9e3779b97f4a7c15ull;
+  x = (x ^ (x >> 30)) * 0xbf58476d1ce4e5b9ull;
+  x = (x ^ (x >> 27)) * 0x94d049bb133111ebull;
+  return x ^ (x >> 31);
+}
 template <int VB>
 __global__ void __cluster_dims__(kSearchCtas) __launch_bounds__(kSearchThreads)
 unnamed_rows_kernel(const SearchArgs a) {
   extern __shared__ unsigned s_bits[];
-  __shared__ unsigned long long s_sums[3];  // rows named, and the two sums
+  __shared__ unsigned long long s_sums[2];  // rows named; mixtures of them less those of all rows
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const auto cluster = cooperative_groups::this_cluster();
   const unsigned rank = cluster.block_rank();
-  if (threadIdx.x < 3) s_sums[threadIdx.x] = 0;
+  if (threadIdx.x < 2) s_sums[threadIdx.x] = 0;
   __syncthreads();
   constexpr int kAtOnce = 16, kStep = kSearchCtas * kSearchThreads;
-  unsigned long long mine[3] = {0, 0, 0};
+  unsigned long long mine[2] = {0, 0};
   for (long long i0 = rank * kSearchThreads + threadIdx.x; i0 < a.total; i0 += kStep * kAtOnce) {
     int p[kAtOnce];
 #pragma unroll
@@ -157,24 +164,24 @@ unnamed_rows_kernel(const SearchArgs a) {
 #pragma unroll
     for (int u = 0; u < kAtOnce; u++) {
       const unsigned row = (unsigned)(p[u] >= 0 ? p[u] : -2 - p[u]);
+      if (i0 + u * kStep < a.total) mine[1] -= mixed((unsigned)(i0 + u * kStep));
       if (row >= a.total) continue;  // -1, or outside
       mine[0]++;
-      mine[1] += row;
-      mine[2] += (unsigned long long)row * row;
+      mine[1] += mixed(row);
     }
   }
 #pragma unroll
-  for (int i = 0; i < 3; i++) {
+  for (int i = 0; i < 2; i++) {
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) mine[i] += __shfl_xor_sync(0xffffffffu, mine[i], d);
     if ((threadIdx.x & 31) == 0) atomicAdd(&s_sums[i], mine[i]);
   }
   cluster.sync();
-  unsigned long long all[3] = {0, 0, 0};
+  unsigned long long all[2] = {0, 0};
   for (unsigned r = 0; r < kSearchCtas; r++)
-    for (int i = 0; i < 3; i++) all[i] += cluster.map_shared_rank(s_sums, r)[i];
+    for (int i = 0; i < 2; i++) all[i] += cluster.map_shared_rank(s_sums, r)[i];
   cluster.sync();  // nobody leaves while others read its sums
-  if (all[0] == (unsigned long long)a.total && all[1] == a.sum && all[2] == a.squares) return;
+  if (all[0] == (unsigned long long)a.total && all[1] == 0) return;
   for (long long from = (long long)rank * a.window; from < a.total;
        from += (long long)kSearchCtas * a.window) {
     clear_unnamed<VB>(s_bits, (unsigned)from, (unsigned)min((long long)a.window, a.total - from),
@@ -483,9 +490,6 @@ int search_unnamed(Unnamed* u, const int* places, long long total, unsigned char
   a.scales = scales;
   a.total = total;
   a.row_bytes = row_bytes;
-  const unsigned __int128 n = (unsigned __int128)total;
-  a.sum = (unsigned long long)(n * (n - 1) / 2);
-  a.squares = (unsigned long long)(n * (n - 1) * (2 * n - 1) / 6);
   a.window = (unsigned)round_up((size_t)((total + kSearchCtas - 1) / kSearchCtas), 32);
   if (a.window > kMostWindow) a.window = kMostWindow;
   unnamed_rows_kernel<VB><<<kSearchCtas, kSearchThreads, a.window / 8, st>>>(a);

@@ -141,3 +141,19 @@ def test_more_rows_than_the_windows_of_one_search():
     want[places[t, j].long()] = x[t]
     foul(want.numel() * 2)
     assert torch.equal(R.sort_cells(x, places), want)
+
+
+@pytest.mark.parametrize("T", [4000, 20000])
+def test_rows_named_twice_in_place_of_others_with_the_same_sums(T):
+    """0, 3, 5 and 6 have the sum and the squares' sum of 1, 2, 4 and 7."""
+    from brainstorm_b200._C import router as R
+
+    k, d = 2, 64
+    places, _ = R.order_picks(torch.randint(0, 5, (T, k), device="cuda"), 5)
+    flat = places.view(-1)
+    for a, b in ((0, 1), (3, 2), (5, 4), (6, 7)):
+        flat[flat == a] = b
+    x = torch.randn(T, d, device="cuda")
+    foul(T * k * d * 4)
+    got = R.sort_cells(x, places)
+    assert bool((got[[0, 3, 5, 6]] == 0).all()) and bool(torch.isfinite(got).all())
