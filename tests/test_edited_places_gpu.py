@@ -157,3 +157,46 @@ def test_rows_named_twice_in_place_of_others_with_the_same_sums(T):
     foul(T * k * d * 4)
     got = R.sort_cells(x, places)
     assert bool((got[[0, 3, 5, 6]] == 0).all()) and bool(torch.isfinite(got).all())
+
+
+def test_captured_training_pass_over_edited_places():
+    """More rows than one CTA searches: the search beside the kernels that move rows, replayed with other
+    picks and other edits."""
+    from brainstorm_b200._C import router as R
+
+    T, k, E, d = 6000, 3, 12, 96
+    gen = torch.Generator(device="cuda").manual_seed(3)
+
+    def fresh():
+        return (torch.randint(-1, E, (T, k), device="cuda", generator=gen),
+                torch.rand(T, k, device="cuda", generator=gen) < 0.2,
+                torch.randn(T, d, device="cuda", generator=gen).bfloat16(),
+                torch.rand(T, k, device="cuda", generator=gen),
+                torch.randn(T, d, device="cuda", generator=gen).bfloat16())
+
+    held = fresh()
+
+    def step(picks, cut, x, gates, gy):
+        x, gates = x.detach().requires_grad_(), gates.detach().requires_grad_()
+        places, _ = R.order_picks(picks, E)
+        places = torch.where(cut, -1, places)
+        rows = R.sort_cells(x, places)
+        leaf = rows.detach().requires_grad_()
+        out = R.unsort_cells(leaf, places, gates)
+        grads = torch.autograd.grad(out, (leaf, gates), gy)
+        return (rows.detach(), out.detach()) + grads + torch.autograd.grad(rows, (x,), grads[0])
+
+    step(*held)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(*held)
+    for _ in range(4):
+        for a, b in zip(held, fresh()):
+            a.copy_(b)
+        for a in got:
+            a.view(torch.uint8).fill_(0xff)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, step(*held)):
+            assert torch.equal(a, b) and bool(torch.isfinite(a).all())

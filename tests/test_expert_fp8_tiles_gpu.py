@@ -156,3 +156,48 @@ def test_layer_of_all_operators_within_twice_the_codes_error():
         a, b = a.detach().double(), b.detach().double()
         off = float((a - b).norm() / b.norm())
         assert off < 2 * expected[name], (name, off, expected[name])
+
+
+@pytest.mark.parametrize("padded", [False, True])
+def test_loads_beyond_the_buffer_and_below_zero_are_cut(padded):
+    """Loads are on the device and not checked: no row outside the buffer, or outside its slot, is read or
+    written."""
+    from brainstorm_b200._C import expert as X
+
+    E, N, K = 4, 144, 272
+    slot = 70 if padded else 0
+    L = slot * E if padded else 300
+    given = [40, -3, 2 ** 31 - 1, 2 ** 31 - 1]
+    real = [40, 0, 70, 70] if padded else [40, 0, 260, 0]
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(L, K, device="cuda", generator=gen).bfloat16()
+    g = torch.randn(L, N, device="cuda", generator=gen).bfloat16()
+    rows, rs = X.quantize_rows(x)
+    w, ws = X.quantize_expert_weights(torch.randn(E, N, K, device="cuda", generator=gen))
+    counts, cut = (torch.tensor(n, dtype=torch.int32, device="cuda") for n in (given, real))
+    for zero in (False, True):
+        outs = []
+        for loads in (counts, cut):
+            out = torch.full((L, N), 7.0, dtype=torch.bfloat16, device="cuda")
+            outs.append(X.grouped_expert_linear_fp8(rows, rs, w, ws, loads, padded, slot, out=out,
+                                                    zero_unused=zero))
+        assert torch.equal(*outs)
+    assert torch.equal(X.grouped_expert_weight_grad(g, x, counts, padded, slot),
+                       X.grouped_expert_weight_grad(g, x, cut, padded, slot))
+    X.check_status()
+
+
+@pytest.mark.parametrize("padded", [False, True])
+def test_no_expert_has_a_row(padded):
+    from brainstorm_b200._C import expert as X
+
+    E, N, K, L = 5, 272, 144, 500
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    x = torch.randn(L, K, device="cuda", generator=gen).bfloat16()
+    loads = torch.zeros(E, dtype=torch.int32, device="cuda")
+    w = torch.randn(E, N, K, device="cuda", generator=gen).requires_grad_()
+    x.requires_grad_()
+    out = X.expert_linear_fp8(x, w, loads, padded)
+    grads = torch.autograd.grad(out, (x, w), torch.full_like(out, float("nan")))
+    X.check_status()
+    assert bool((out == 0).all()) and all(bool((t == 0).all()) for t in grads)
